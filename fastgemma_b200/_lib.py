@@ -71,6 +71,18 @@ SIGNATURES = {
                            _p, _sz, _p, _sz, _p, _sz, _p, _sz, _p], _i),
     "fgm_cuda_qkv_post_cs": ([_p, _i, _p, _p, _i, _i, _i, _i, _i, _p, _p, C.c_float, _p, _p, _i,
                               _p, _i, _i, _p, _sz, _p, _sz, _p, _sz, _p, _sz, _p], _i),
+    "fgm_cuda_tree_mask": ([_p, _p, _p, _p, _i, _i, _p], _i),
+    "fgm_cuda_attend_workspace": ([_p, _i, _i], _sz),
+    "fgm_cuda_attend_tree_q8": ([_p, _p, _i, _i, _i, _p, _p, _p, _i, _p, _i, _p, _sz, _sz, _p, _sz,
+                                 _p], _i),
+    "fgm_cuda_attend_accum_q8": ([_p, _p, _i, _i, _i, _p, _p, _p, _i, _p, _sz, _sz, _p, C.c_float,
+                                  _p, _sz, _p], _i),
+    "fgm_cuda_attend_acc_q8": ([_p, _p, _i, _i, _p, C.c_float, _p, _i, _p, _sz, _p], _i),
+    "fgm_cuda_tree_verify": ([_p, _p, _p, _p, _p, _p, _i, _i, _p], _i),
+    "fgm_cuda_kv_accept": ([_p, _i, _i, _p, _p, _p, _p, _p], _i),
+    "fgm_cuda_kv_evict_q8": ([_p, _p, _i, _i, _i, _p, _p, _p, _p, _sz, _p], _i),
+    "fgm_cuda_qkv_post_tree": ([_p, _p, _i, _p, _p, _i, _i, _i, _p, _p, C.c_float, _p, _p, _i, _p,
+                                _p, _p], _i),
     "fgm_cuda_ipc_alloc": ([_sz, C.POINTER(_p)], _i),
     "fgm_cuda_ipc_free": ([_p], _i),
     "fgm_cuda_ipc_handle": ([_p, _p], _i),

@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <climits>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -1674,11 +1675,240 @@ int fgm_cuda_qkv_post_cs(float *q, int q_ld, float *k, float *v, int kv_ld, int 
   if (rc) return rc;
   QkvParams p{q, k, v, q_ld, kv_ld, n_heads, kv_heads, head_dim, q_norm, k_norm, eps, inv_freq,
               pos, ring, cap, kc, ks, vt, vs, kc_stride, ks_stride, vt_stride, vs_stride,
-              positions > 0 ? cs : nullptr, positions};
+              positions > 0 ? cs : nullptr, positions, 1, nullptr, nullptr, 0};
   if (qkv_post_smem(p) > di->smem_optin)
     return fail(FGM_CUDA_EINVAL, "qkv_post: %d heads of %d need too much shared memory",
                 n_heads + 2 * kv_heads, head_dim);
   return glue_done(launch_qkv_post(p, rows, glue_pdl(), (cudaStream_t)stream), "qkv_post launch");
+}
+
+// --------------------------- several tokens per sequence over one KV cache
+static uintptr_t addr(const void *p) { return reinterpret_cast<uintptr_t>(p); }
+
+static int check_kv(const char *who, const fgm_cuda_kv *kv) {
+  if (!kv) return fail(FGM_CUDA_EINVAL, "%s: null pointer", who);
+  if (kv->rows < 0 || kv->rows > 65535 || kv->kv_heads <= 0 || kv->kv_heads > 128 ||
+      kv->head_dim <= 0 || kv->head_dim % 64 != 0 || kv->head_dim > 512)
+    return fail(FGM_CUDA_EINVAL,
+                "%s: rows=%d kv_heads=%d head_dim=%d (need rows <= 65535, kv_heads <= 128, head_dim "
+                "a multiple of 64, at most 512)", who, kv->rows, kv->kv_heads, kv->head_dim);
+  if (kv->cap <= 0 || kv->cap > (1 << 30) || kv->ring < 0 || kv->ring > kv->cap)
+    return fail(FGM_CUDA_EINVAL, "%s: cap=%d ring=%d (need 0 < cap <= 2^30, ring <= cap)", who,
+                kv->cap, kv->ring);
+  if (kv->rows == 0) return FGM_CUDA_OK;
+  if (!kv->kc || !kv->ks || !kv->vt || !kv->vs)
+    return fail(FGM_CUDA_EINVAL, "%s: null pointer in the cache", who);
+  if ((addr(kv->kc) | addr(kv->vt) | kv->kc_stride | kv->vt_stride) & 15)
+    return fail(FGM_CUDA_EINVAL, "%s: kc and vt must be 16-byte aligned, their strides multiples "
+                "of 16", who);
+  if ((addr(kv->ks) | addr(kv->vs) | addr(kv->acc) | addr(kv->tpos)) & 3)
+    return fail(FGM_CUDA_EINVAL, "%s: ks, vs, acc and tpos must be 4-byte aligned", who);
+  const size_t cap = (size_t)kv->cap, kvd = (size_t)kv->kv_heads * kv->head_dim;
+  if (kv->rows > 1 &&
+      (kv->kc_stride < cap * kvd || kv->vt_stride < ((cap + 3) & ~(size_t)3) * kvd ||
+       kv->ks_stride < cap || kv->vs_stride < cap || (kv->acc && kv->acc_stride < cap) ||
+       (kv->tpos && kv->tpos_stride < cap)))
+    return fail(FGM_CUDA_EINVAL, "%s: strides shorter than %d cache slots", who, kv->cap);
+  return FGM_CUDA_OK;
+}
+
+static int check_tree(const char *who, const fgm_cuda_kv *kv, int n_heads, int T) {
+  const int rc = check_kv(who, kv);
+  if (rc) return rc;
+  if (T < 1 || T > FGM_CUDA_TREE_MAX || T > kv->cap)
+    return fail(FGM_CUDA_EINVAL, "%s: T=%d (need 1 <= T <= %d and T <= cap=%d)", who, T,
+                FGM_CUDA_TREE_MAX, kv->cap);
+  if (n_heads <= 0 || n_heads % kv->kv_heads != 0 || n_heads / kv->kv_heads > 16)
+    return fail(FGM_CUDA_EINVAL, "%s: heads=%d kv_heads=%d (need a multiple, at most 16 per KV head)",
+                who, n_heads, kv->kv_heads);
+  if ((long long)kv->rows * T > INT_MAX / 2)
+    return fail(FGM_CUDA_EINVAL, "%s: rows=%d T=%d", who, kv->rows, T);
+  return FGM_CUDA_OK;
+}
+
+// The contract that the three attention entries share; out and out_ld only
+// where has_out.
+static int check_attend(const char *who, const TreeParams &p, size_t ws_bytes, bool has_out) {
+  const fgm_cuda_kv &kv = p.kv;
+  const int width = p.n_heads * kv.head_dim;
+  if (p.q_ld < width || p.q_ld % 4 != 0 || (has_out && (p.out_ld < width || p.out_ld % 4 != 0)))
+    return fail(FGM_CUDA_EINVAL, "%s: q_ld=%d out_ld=%d (need multiples of 4, at least %d)", who,
+                p.q_ld, p.out_ld, width);
+  if (p.window < 0) return fail(FGM_CUDA_EINVAL, "%s: window=%d", who, p.window);
+  if (kv.ring && (p.window < 1 || (long long)p.window + p.T - 1 > kv.ring))
+    return fail(FGM_CUDA_EINVAL, "%s: ring=%d window=%d T=%d (a ring needs 0 < window and window + "
+                "T - 1 <= ring)", who, kv.ring, p.window, p.T);
+  if (kv.rows == 0) return FGM_CUDA_OK;
+  if (!p.q || !p.lens || (has_out && !p.out) || !p.ws)
+    return fail(FGM_CUDA_EINVAL, "%s: null pointer", who);
+  if ((addr(p.q) | (has_out ? addr(p.out) : 0)) & 15)
+    return fail(FGM_CUDA_EINVAL, "%s: q and out must be 16-byte aligned", who);
+  if (addr(p.ws) & 255) return fail(FGM_CUDA_EINVAL, "%s: ws must be 256-byte aligned", who);
+  if (addr(p.mask) & 7) return fail(FGM_CUDA_EINVAL, "%s: mask must be 8-byte aligned", who);
+  const size_t need = attend_workspace(kv, p.n_heads, p.T);
+  if (ws_bytes < need)
+    return fail(FGM_CUDA_EINVAL, "%s: ws_bytes=%zu, need %zu", who, ws_bytes, need);
+  return FGM_CUDA_OK;
+}
+
+int fgm_cuda_tree_mask(uint64_t *mask, int32_t *pos, const int32_t *parent, const int32_t *lens,
+                       int rows, int T, void *stream) {
+  if (rows < 0 || rows > 65535 || T < 1 || T > FGM_CUDA_TREE_MAX)
+    return fail(FGM_CUDA_EINVAL, "tree_mask: rows=%d T=%d (need T <= %d)", rows, T,
+                FGM_CUDA_TREE_MAX);
+  if (rows == 0) return FGM_CUDA_OK;
+  if (!mask || !parent || (pos && !lens)) return fail(FGM_CUDA_EINVAL, "tree_mask: null pointer");
+  return glue_done(launch_tree_mask(mask, pos, parent, lens, rows, T, (cudaStream_t)stream),
+                   "tree_mask launch");
+}
+
+size_t fgm_cuda_attend_workspace(const fgm_cuda_kv *kv, int n_heads, int T) {
+  if (check_tree("attend_workspace", kv, n_heads, T)) return 0;
+  return attend_workspace(*kv, n_heads, T);
+}
+
+int fgm_cuda_attend_tree_q8(const fgm_cuda_kv *kv, const float *q, int q_ld, int n_heads, int T,
+                            const int32_t *lens, const uint64_t *mask, const int32_t *pos,
+                            int window, float *out, int out_ld, float *lse, size_t lse_row,
+                            size_t lse_head, void *ws, size_t ws_bytes, void *stream) {
+  int rc = check_tree("attend_tree", kv, n_heads, T);
+  if (rc) return rc;
+  const TreeParams p{*kv, q, q_ld, n_heads, T, lens, mask, pos, window, out, out_ld, lse, lse_row,
+                     lse_head, nullptr, 0.0f, ws};
+  if ((rc = check_attend("attend_tree", p, ws_bytes, true)) || kv->rows == 0) return rc;
+  DevInfo *di = nullptr;
+  if ((rc = dev_info(&di))) return rc;
+  return glue_done(launch_attend_tree(p, di->sms, (cudaStream_t)stream), "attend_tree launch");
+}
+
+int fgm_cuda_attend_accum_q8(const fgm_cuda_kv *kv, const float *q, int q_ld, int n_heads, int T,
+                             const int32_t *lens, const uint64_t *mask, const int32_t *pos,
+                             int window, const float *lse, size_t lse_row, size_t lse_head,
+                             const uint8_t *take, float decay, void *ws, size_t ws_bytes,
+                             void *stream) {
+  int rc = check_tree("attend_accum", kv, n_heads, T);
+  if (rc) return rc;
+  const TreeParams p{*kv, q, q_ld, n_heads, T, lens, mask, pos, window, nullptr, 0,
+                     const_cast<float *>(lse), lse_row, lse_head, take, decay, ws};
+  if ((rc = check_attend("attend_accum", p, ws_bytes, false)) || kv->rows == 0) return rc;
+  if (!lse || !kv->acc) return fail(FGM_CUDA_EINVAL, "attend_accum: null pointer (lse, kv->acc)");
+  DevInfo *di = nullptr;
+  if ((rc = dev_info(&di))) return rc;
+  return glue_done(launch_attend_accum(p, di->sms, (cudaStream_t)stream), "attend_accum launch");
+}
+
+int fgm_cuda_attend_acc_q8(const fgm_cuda_kv *kv, const float *q, int q_ld, int n_heads,
+                           const int32_t *lens, float decay, float *out, int out_ld, void *ws,
+                           size_t ws_bytes, void *stream) {
+  int rc = check_tree("attend_acc", kv, n_heads, 1);
+  if (rc) return rc;
+  if (kv->ring) return fail(FGM_CUDA_EINVAL, "attend_acc: ring=%d (linear caches only)", kv->ring);
+  const TreeParams p{*kv, q, q_ld, n_heads, 1, lens, nullptr, nullptr, 0, out, out_ld, nullptr,
+                     0, 0, nullptr, decay, ws};
+  if ((rc = check_attend("attend_acc", p, ws_bytes, true)) || kv->rows == 0) return rc;
+  if (!kv->acc) return fail(FGM_CUDA_EINVAL, "attend_acc: null pointer (kv->acc)");
+  DevInfo *di = nullptr;
+  if ((rc = dev_info(&di))) return rc;
+  rc = glue_done(launch_attend_acc(p, di->sms, (cudaStream_t)stream), "attend_acc launch");
+  if (!rc) count_launch();
+  return rc;
+}
+
+int fgm_cuda_tree_verify(int32_t *path, int32_t *n_acc, int32_t *next, const int32_t *parent,
+                         const int32_t *token, const int32_t *target, int rows, int T,
+                         void *stream) {
+  if (rows < 0 || rows > 65535 || T < 1 || T > FGM_CUDA_TREE_MAX)
+    return fail(FGM_CUDA_EINVAL, "tree_verify: rows=%d T=%d (need T <= %d)", rows, T,
+                FGM_CUDA_TREE_MAX);
+  if (rows == 0) return FGM_CUDA_OK;
+  if (!path || !n_acc || !next || !parent || !token || !target)
+    return fail(FGM_CUDA_EINVAL, "tree_verify: null pointer");
+  return glue_done(launch_tree_verify(path, n_acc, next, parent, token, target, rows, T,
+                                      (cudaStream_t)stream),
+                   "tree_verify launch");
+}
+
+int fgm_cuda_kv_accept(const fgm_cuda_kv *kv, int layers, int T, const int32_t *lens,
+                       const int32_t *path, const int32_t *n_acc, int32_t *lens_new,
+                       void *stream) {
+  if (layers < 0) return fail(FGM_CUDA_EINVAL, "kv_accept: layers=%d", layers);
+  if (layers == 0) return FGM_CUDA_OK;
+  for (int l = 0; l < layers; l++) {
+    const int rc = check_kv("kv_accept", kv ? kv + l : nullptr);
+    if (rc) return rc;
+    if (kv[l].rows != kv[0].rows)
+      return fail(FGM_CUDA_EINVAL, "kv_accept: layer %d has rows=%d, layer 0 %d", l, kv[l].rows,
+                  kv[0].rows);
+    if (T < 1 || T > FGM_CUDA_TREE_MAX || T > (kv[l].ring ? kv[l].ring : kv[l].cap))
+      return fail(FGM_CUDA_EINVAL, "kv_accept: T=%d (need 1 <= T <= %d, within the cache)", T,
+                  FGM_CUDA_TREE_MAX);
+  }
+  if (kv->rows == 0) return FGM_CUDA_OK;
+  if (!lens || !path || !n_acc) return fail(FGM_CUDA_EINVAL, "kv_accept: null pointer");
+  if (lens_new == lens)
+    return fail(FGM_CUDA_EINVAL, "kv_accept: lens_new must not be lens (layers read it)");
+  int launches = 0;
+  const cudaError_t e = launch_kv_accept(kv, layers, T, lens, path, n_acc, lens_new, &launches,
+                                         (cudaStream_t)stream);
+  count_launch(launches);
+  return e == cudaSuccess ? FGM_CUDA_OK : cuda_fail(e, "kv_accept launch");
+}
+
+int fgm_cuda_kv_evict_q8(const fgm_cuda_kv *kv, const int32_t *lens, int budget, int sink,
+                         int recent, int32_t *map, int32_t *lens_out, float *acc_out,
+                         int32_t *tpos_out, size_t out_stride, void *stream) {
+  int rc = check_kv("kv_evict", kv);
+  if (rc) return rc;
+  if (kv->ring || kv->cap > 524288)
+    return fail(FGM_CUDA_EINVAL, "kv_evict: ring=%d cap=%d (linear caches of at most 524288 slots)",
+                kv->ring, kv->cap);
+  if (budget < 1 || budget > kv->cap || sink < 0 || recent < 0)
+    return fail(FGM_CUDA_EINVAL, "kv_evict: budget=%d sink=%d recent=%d (need 1 <= budget <= cap=%d, "
+                "sink, recent >= 0)", budget, sink, recent, kv->cap);
+  if ((acc_out || tpos_out) && kv->rows > 1 && out_stride < (size_t)budget)
+    return fail(FGM_CUDA_EINVAL, "kv_evict: out_stride=%zu < budget=%d", out_stride, budget);
+  if (kv->rows == 0) return FGM_CUDA_OK;
+  if (!lens || !map || !lens_out || !kv->acc)
+    return fail(FGM_CUDA_EINVAL, "kv_evict: null pointer (lens, map, lens_out, kv->acc)");
+  rc = glue_done(launch_kv_evict(*kv, lens, budget, sink, recent, map, lens_out, acc_out, tpos_out,
+                                 out_stride, (cudaStream_t)stream),
+                 "kv_evict launch");
+  if (!rc) count_launch();
+  return rc;
+}
+
+int fgm_cuda_qkv_post_tree(const fgm_cuda_kv *kv, float *q, int q_ld, float *k, float *v, int kv_ld,
+                           int n_heads, int T, const float *q_norm, const float *k_norm, float eps,
+                           const float *inv_freq, const float *cs, int positions,
+                           const int32_t *pos, const int32_t *lens, void *stream) {
+  int rc = check_tree("qkv_post_tree", kv, n_heads, T);
+  if (rc) return rc;
+  if (positions < 0 || (positions > 0 && !cs))
+    return fail(FGM_CUDA_EINVAL, "qkv_post_tree: rope table of %d positions at %p", positions,
+                (const void *)cs);
+  const int hd = kv->head_dim;
+  if (n_heads + 2 * kv->kv_heads > 48 || q_ld < n_heads * hd || kv_ld < kv->kv_heads * hd ||
+      q_ld % 4 != 0 || kv_ld % 4 != 0)
+    return fail(FGM_CUDA_EINVAL, "qkv_post_tree: heads=%d kv_heads=%d head_dim=%d q_ld=%d kv_ld=%d",
+                n_heads, kv->kv_heads, hd, q_ld, kv_ld);
+  if (kv->ring && T > kv->ring)
+    return fail(FGM_CUDA_EINVAL, "qkv_post_tree: T=%d ring=%d", T, kv->ring);
+  if (kv->rows == 0) return FGM_CUDA_OK;
+  if (!q || !k || !v || !q_norm || !k_norm || !inv_freq || !pos || !lens)
+    return fail(FGM_CUDA_EINVAL, "qkv_post_tree: null pointer");
+  if ((addr(q) | addr(k) | addr(v)) & 15)
+    return fail(FGM_CUDA_EINVAL, "qkv_post_tree: q, k and v must be 16-byte aligned");
+  DevInfo *di = nullptr;
+  if ((rc = dev_info(&di))) return rc;
+  const QkvParams p{q, k, v, q_ld, kv_ld, n_heads, kv->kv_heads, hd, q_norm, k_norm, eps, inv_freq,
+                    pos, kv->ring, kv->cap, kv->kc, kv->ks, kv->vt, kv->vs, kv->kc_stride,
+                    kv->ks_stride, kv->vt_stride, kv->vs_stride, positions > 0 ? cs : nullptr,
+                    positions, T, lens, kv->tpos, kv->tpos_stride};
+  if (qkv_post_smem(p) > di->smem_optin)
+    return fail(FGM_CUDA_EINVAL, "qkv_post_tree: %d heads of %d need too much shared memory",
+                n_heads + 2 * kv->kv_heads, hd);
+  return glue_done(launch_qkv_post(p, kv->rows * T, glue_pdl(), (cudaStream_t)stream),
+                   "qkv_post_tree launch");
 }
 
 // ------------------------------------------------ peer memory, fused gather

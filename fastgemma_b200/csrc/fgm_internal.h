@@ -8,6 +8,8 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include "fgm_cuda.h"
+
 namespace fgm {
 
 constexpr int kMaxGatherRanks = 8;
@@ -150,6 +152,10 @@ struct QkvParams {
   size_t kc_stride, ks_stride, vt_stride, vs_stride;  // per row (elements)
   const float *rope_tab;            // host-computed cos | sin per position, or null
   int rope_positions;               // positions in rope_tab
+  int T;                            // rows per cache: row r's cache is r / T
+  const int32_t *lens;              // slot of position lens[r / T] + r % T (null: pos[r])
+  int32_t *tpos;                    // token position per slot, or null
+  size_t tpos_stride;
 };
 size_t qkv_post_smem(const QkvParams &p);
 cudaError_t launch_qkv_post(const QkvParams &p, int rows, bool pdl, cudaStream_t st);
@@ -162,6 +168,39 @@ cudaError_t launch_attend_q8(const AttnParams &p, int rows, bool pdl, size_t sme
 // device memory with one kernel.
 cudaError_t launch_pull(const void *s1, void *d1, size_t n1, const void *s2, void *d2, size_t n2,
                         bool pdl, cudaStream_t st);
+
+// ---- several tokens per sequence over one KV cache (kvattn.cu, kvcache.cu)
+struct TreeParams {
+  fgm_cuda_kv kv;
+  const float *q;
+  int q_ld, n_heads, T;
+  const int32_t *lens;
+  const uint64_t *mask;   // [rows][T][(T + 63) / 64], or null: the nodes before
+  const int32_t *pos;     // [rows * T], or null: lens + i
+  int window;
+  float *out;
+  int out_ld;
+  float *lse;             // row r, head h at r * lse_row + h * lse_head; read by the accumulation
+  size_t lse_row, lse_head;
+  const uint8_t *take;    // [rows * T], or null: all
+  float decay;
+  void *ws;
+};
+size_t attend_workspace(const fgm_cuda_kv &kv, int n_heads, int T);
+cudaError_t launch_attend_tree(const TreeParams &p, int num_sms, cudaStream_t st);
+cudaError_t launch_attend_accum(const TreeParams &p, int num_sms, cudaStream_t st);
+cudaError_t launch_attend_acc(const TreeParams &p, int num_sms, cudaStream_t st);
+cudaError_t launch_tree_mask(uint64_t *mask, int32_t *pos, const int32_t *parent,
+                             const int32_t *lens, int rows, int T, cudaStream_t st);
+cudaError_t launch_tree_verify(int32_t *path, int32_t *n_acc, int32_t *next, const int32_t *parent,
+                               const int32_t *token, const int32_t *target, int rows, int T,
+                               cudaStream_t st);
+cudaError_t launch_kv_accept(const fgm_cuda_kv *kv, int layers, int T, const int32_t *lens,
+                             const int32_t *path, const int32_t *n_acc, int32_t *lens_new,
+                             int *launches, cudaStream_t st);
+cudaError_t launch_kv_evict(const fgm_cuda_kv &kv, const int32_t *lens, int budget, int sink,
+                            int recent, int32_t *map, int32_t *lens_out, float *acc_out,
+                            int32_t *tpos_out, size_t out_stride, cudaStream_t st);
 
 // ----------------------------------------------------------- tensor cores
 struct TcParams {

@@ -1110,7 +1110,9 @@ __global__ void __launch_bounds__(kGlueThreads) qkv_post_kernel(const QkvParams 
     }
   }
   // int8 K and V rows with one scale each (ops.c:181-204), into the caches
-  const int slot = p.ring ? pos % p.ring : pos;
+  const int c = r / p.T;  // its cache; the nodes of a tree share one
+  const int at = p.lens ? p.lens[c] + (r - c * p.T) : pos;
+  const int slot = p.ring ? at % p.ring : at;
   if (slot < 0 || slot >= p.cap) return;  // no cache entry for this row (whole CTA)
   kmx = warp_max(kmx);
   vmx = warp_max(vmx);
@@ -1128,15 +1130,16 @@ __global__ void __launch_bounds__(kGlueThreads) qkv_post_kernel(const QkvParams 
   const float vsc = vmx == 0.0f ? 1.0f : __fdiv_rn(vmx, 127.0f);
   const float kinv = __fdiv_rn(1.0f, ksc), vinv = __fdiv_rn(1.0f, vsc);
   const float *xk = xs + nq, *xv = xs + nq + kvd;
-  int8_t *kd = p.kc + (size_t)r * p.kc_stride + (size_t)slot * kvd;
-  int8_t *vd = p.vt + (size_t)r * p.vt_stride + (size_t)(slot >> 2) * kvd * 4 + (slot & 3);
+  int8_t *kd = p.kc + (size_t)c * p.kc_stride + (size_t)slot * kvd;
+  int8_t *vd = p.vt + (size_t)c * p.vt_stride + (size_t)(slot >> 2) * kvd * 4 + (slot & 3);
   for (int i = threadIdx.x; i < kvd; i += blockDim.x) {
     kd[i] = (int8_t)q8_x86(__fmul_rn(xk[i], kinv));
     vd[(size_t)i * 4] = (int8_t)q8_x86(__fmul_rn(xv[i], vinv));
   }
   if (threadIdx.x == 0) {
-    p.ks[(size_t)r * p.ks_stride + slot] = ksc;
-    p.vs[(size_t)r * p.vs_stride + slot] = vsc;
+    p.ks[(size_t)c * p.ks_stride + slot] = ksc;
+    p.vs[(size_t)c * p.vs_stride + slot] = vsc;
+    if (p.tpos) p.tpos[(size_t)c * p.tpos_stride + slot] = pos;
   }
 }
 

@@ -210,6 +210,162 @@ def qkv_post(q, k, v, rows, n_heads, kv_heads, head_dim, q_norm, k_norm, eps, in
          ks_stride, _p(vt), vt_stride, _p(vs), vs_stride, _s(stream))
 
 
+# ----------------------------- several tokens per sequence over one KV cache
+class KvCache(C.Structure):
+    """One layer's int8 KV caches of several sequences (fgm_cuda_kv): a view of
+    tensors the caller owns, kept alive by it.
+
+    kc [rows][cap][kv_heads * head_dim] int8, ks / vs [rows][cap] f32, vt
+    [rows][ceil(cap / 4) * 4 * kv_heads * head_dim] int8 in any shape after
+    the first dimension, acc [rows][cap] f32 and tpos [rows][cap] int32 where
+    used; rows may be strided, what lies behind a row is contiguous."""
+    _fields_ = [("kc", C.c_void_p), ("ks", C.c_void_p), ("vt", C.c_void_p), ("vs", C.c_void_p),
+                ("acc", C.c_void_p), ("tpos", C.c_void_p),
+                ("kc_stride", C.c_size_t), ("ks_stride", C.c_size_t), ("vt_stride", C.c_size_t),
+                ("vs_stride", C.c_size_t), ("acc_stride", C.c_size_t), ("tpos_stride", C.c_size_t),
+                ("rows", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int),
+                ("cap", C.c_int), ("ring", C.c_int)]
+
+    def __init__(self, kc, ks, vt, vs, kv_heads, head_dim, ring=0, acc=None, tpos=None):
+        super().__init__()
+        rows, cap = kc.shape[0], kc.shape[1]
+        kvd = kv_heads * head_dim
+        if tuple(kc.shape) != (rows, cap, kvd):
+            raise ValueError(f"kc has shape {tuple(kc.shape)}, not [rows][cap][{kvd}]")
+        for name, t, dtype, n in (("kc", kc, torch.int8, cap * kvd), ("ks", ks, torch.float32, cap),
+                                  ("vt", vt, torch.int8, (cap + 3) // 4 * 4 * kvd),
+                                  ("vs", vs, torch.float32, cap), ("acc", acc, torch.float32, cap),
+                                  ("tpos", tpos, torch.int32, cap)):
+            if t is None:
+                continue
+            if t.dtype != dtype or t.shape[0] != rows or (rows and t[0].numel() < n):
+                raise ValueError(f"{name}: {t.dtype} {tuple(t.shape)}, need {dtype} with {n} "
+                                 f"elements in each of {rows} rows")
+            if rows and not t[0].is_contiguous():
+                raise ValueError(f"{name}: a row has to be contiguous")
+            setattr(self, name, t.data_ptr())
+            setattr(self, name + "_stride", t.stride(0))
+        self.rows, self.kv_heads, self.head_dim, self.cap, self.ring = (rows, kv_heads, head_dim,
+                                                                        cap, ring)
+        self._keep = (kc, ks, vt, vs, acc, tpos)
+
+
+def kv_layers(views):
+    """Several layers' KvCache views as one array for kv_accept."""
+    arr = (KvCache * len(views))(*views)
+    arr._keep_views = list(views)
+    return arr
+
+
+def _flat(**tensors):
+    """The entries take whole tensors by address: a strided one would be misread."""
+    for name, t in tensors.items():
+        if t is not None and not t.is_contiguous():
+            raise ValueError(f"{name} has to be contiguous")
+
+
+def _lse(lse):
+    return (None, 0, 0) if lse is None else (lse.data_ptr(), lse.stride(0), lse.stride(1))
+
+
+def _on(stream):
+    return torch.cuda.stream(stream or torch.cuda.current_stream())
+
+
+def attend_workspace(kv, n_heads, T):
+    """A workspace for the attention entries on this cache (fgm_cuda_attend_workspace)."""
+    n = call("fgm_cuda_attend_workspace", C.byref(kv), n_heads, T)
+    return torch.empty(max(int(n), 1), dtype=torch.uint8, device="cuda")
+
+
+def _ws(ws, kv, n_heads, T, stream):
+    if ws is None:  # from torch's allocator, on the stream that uses it
+        with _on(stream):
+            ws = attend_workspace(kv, n_heads, T)
+    return ws
+
+
+def tree_mask(mask, pos, parent, lens, stream=None):
+    """Ancestor words mask [rows][T][ceil(T / 64)] (int64) and positions pos
+    [rows * T] of the trees parent [rows][T] (int32)."""
+    rows, T = parent.shape
+    _flat(mask=mask, pos=pos, parent=parent, lens=lens)
+    call("fgm_cuda_tree_mask", _p(mask), _p(pos), _p(parent), _p(lens), rows, T, _s(stream))
+
+
+def attend_tree_q8(out, q, kv, n_heads, T, lens, mask=None, pos=None, window=0, lse=None, ws=None,
+                   q_ld=None, out_ld=None, stream=None):
+    """T nodes of each sequence attend to its cache and to one another (mask
+    None: to the nodes before them); lse [rows * T][n_heads], of any strides, if wanted."""
+    _flat(lens=lens, mask=mask, pos=pos)
+    ws = _ws(ws, kv, n_heads, T, stream)
+    ld = n_heads * kv.head_dim
+    call("fgm_cuda_attend_tree_q8", C.byref(kv), _p(q), ld if q_ld is None else q_ld, n_heads, T,
+         _p(lens), _p(mask), _p(pos), window, _p(out), ld if out_ld is None else out_ld,
+         *_lse(lse), _p(ws), ws.numel(), _s(stream))
+
+
+def attend_accum_q8(q, kv, n_heads, T, lens, lse, mask=None, pos=None, window=0, take=None,
+                    decay=1.0, ws=None, q_ld=None, stream=None):
+    """kv's acc = decay * acc + the weights of the taken nodes (take: uint8
+    [rows * T]) of such an attention, from its lse."""
+    _flat(lens=lens, mask=mask, pos=pos, take=take)
+    ws = _ws(ws, kv, n_heads, T, stream)
+    call("fgm_cuda_attend_accum_q8", C.byref(kv), _p(q),
+         n_heads * kv.head_dim if q_ld is None else q_ld, n_heads, T, _p(lens), _p(mask), _p(pos),
+         window, *_lse(lse), _p(take), decay, _p(ws), ws.numel(), _s(stream))
+
+
+def attend_acc_q8(out, q, kv, n_heads, lens, decay=1.0, ws=None, q_ld=None, out_ld=None,
+                  stream=None):
+    """One token per sequence: attention over slots [0, lens[b]] and its weights added to kv's acc."""
+    ws = _ws(ws, kv, n_heads, 1, stream)
+    ld = n_heads * kv.head_dim
+    call("fgm_cuda_attend_acc_q8", C.byref(kv), _p(q), ld if q_ld is None else q_ld, n_heads,
+         _p(lens), decay, _p(out), ld if out_ld is None else out_ld, _p(ws), ws.numel(),
+         _s(stream))
+
+
+def tree_verify(path, n_acc, next_token, parent, token, target, stream=None):
+    """The accepted path of each drafted tree: path [rows][T] (then -1), its
+    length n_acc and the token after it."""
+    rows, T = parent.shape
+    _flat(path=path, parent=parent, token=token, target=target)
+    call("fgm_cuda_tree_verify", _p(path), _p(n_acc), _p(next_token), _p(parent), _p(token),
+         _p(target), rows, T, _s(stream))
+
+
+def kv_accept(layers, T, lens, path, n_acc, lens_new=None, stream=None):
+    """Move the accepted path's rows behind the committed ones in every layer
+    (layers: kv_layers(...) or one KvCache)."""
+    _flat(lens=lens, path=path, n_acc=n_acc)
+    one = isinstance(layers, KvCache)
+    call("fgm_cuda_kv_accept", C.byref(layers) if one else layers, 1 if one else len(layers), T,
+         _p(lens), _p(path), _p(n_acc), _p(lens_new), _s(stream))
+
+
+def kv_evict_q8(kv, lens, budget, sink, recent, slot_map, lens_out, acc_out=None, tpos_out=None,
+                stream=None):
+    """Keep `budget` slots of each cache (protected, then by accumulated
+    weight); slot_map [rows][budget] says where each slot's row came from."""
+    _flat(lens=lens, slot_map=slot_map, lens_out=lens_out)
+    stride = (acc_out if acc_out is not None else tpos_out).stride(0) \
+        if acc_out is not None or tpos_out is not None else 0
+    if acc_out is not None and tpos_out is not None and tpos_out.stride(0) != stride:
+        raise ValueError("acc_out and tpos_out need the same row stride")
+    call("fgm_cuda_kv_evict_q8", C.byref(kv), _p(lens), budget, sink, recent, _p(slot_map),
+         _p(lens_out), _p(acc_out), _p(tpos_out), stride, _s(stream))
+
+
+def qkv_post_tree(kv, q, k, v, n_heads, T, q_norm, k_norm, eps, inv_freq, pos, lens, q_ld=None,
+                  kv_ld=None, cs=None, stream=None):
+    """qkv_post for the nodes of a tree: rope at pos, K / V rows into slots lens[b] + i."""
+    kvd = kv.kv_heads * kv.head_dim
+    call("fgm_cuda_qkv_post_tree", C.byref(kv), _p(q),
+         n_heads * kv.head_dim if q_ld is None else q_ld, _p(k), _p(v),
+         kvd if kv_ld is None else kv_ld, n_heads, T, _p(q_norm), _p(k_norm), eps, _p(inv_freq),
+         _p(cs), 0 if cs is None else cs.shape[0], _p(pos), _p(lens), _s(stream))
+
 
 # ------------------------------------------------------- decode work list
 class _Work(C.Structure):

@@ -427,6 +427,138 @@ int fgm_cuda_qkv_post_cs(float *q, int q_ld, float *k, float *v, int kv_ld, int 
                          size_t kc_stride, float *ks, size_t ks_stride, int8_t *vt,
                          size_t vt_stride, float *vs, size_t vs_stride, void *stream);
 
+/* --------------------------- several tokens per sequence over one KV cache
+ * Speculative decoding (a tree of drafted tokens verified in one step),
+ * prefill chunks, and a cache held to a budget by the attention its slots
+ * received.  No reference counterpart: the reference attends one token per
+ * call (ops.c:378-640) and drops nothing but a ring's oldest slots.
+ *
+ * One layer's caches of `rows` sequences: K and V as fgm_cuda_attend_q8 reads
+ * and fgm_cuda_qkv_post writes them.  cap: slots of each cache; V holds whole
+ * groups of four.  ring = 0: slot = position; ring > 0 (<= cap): slot =
+ * position % ring.  acc (accumulated attention weight per slot) and tpos (the
+ * token position each slot holds) may be NULL where no entry below needs
+ * them.  Strides count elements from one sequence to the next.  Checked
+ * (EINVAL): head_dim % 64 == 0 and <= 512, kc and vt 16-byte aligned with
+ * strides that are multiples of 16, strides that hold cap slots when rows >
+ * 1.  Slots that no committed token and no node owns are never used: their
+ * bytes and scales may hold anything, not-a-numbers too. */
+typedef struct fgm_cuda_kv {
+  int8_t *kc;   /* K [slot][kv_heads * head_dim] */
+  float *ks;    /* K scales [slot] */
+  int8_t *vt;   /* V [slot / 4][kv_heads * head_dim][slot % 4] */
+  float *vs;    /* V scales [slot] */
+  float *acc;   /* accumulated attention weight [slot], or NULL */
+  int32_t *tpos; /* token position of each slot, or NULL */
+  size_t kc_stride, ks_stride, vt_stride, vs_stride, acc_stride, tpos_stride;
+  int rows, kv_heads, head_dim, cap, ring;
+} fgm_cuda_kv;
+
+#define FGM_CUDA_TREE_MAX 256
+
+/* Ancestor masks and positions of drafted trees.  parent [rows][T]: each
+ * node's parent, an index below its own (node 0, the last chosen token, is
+ * the root; anything else outside [0, i) makes node i a root of its own).
+ * mask [rows][T][(T + 63) / 64]: bit j of node i is set when j is i or one
+ * of its ancestors.  pos [rows * T] (may be NULL): lens[row] + depth. */
+int fgm_cuda_tree_mask(uint64_t *mask, int32_t *pos, const int32_t *parent, const int32_t *lens,
+                       int rows, int T, void *stream);
+
+/* Bytes of workspace that the attention entries below need for this cache,
+ * head count and T (any ws of at least that size, 256-byte aligned; nothing
+ * in it has to be kept or cleared between calls). */
+size_t fgm_cuda_attend_workspace(const fgm_cuda_kv *kv, int n_heads, int T);
+
+/* T tokens ("nodes") of each sequence attend to its cache and to one another.
+ * lens [rows] (device): committed tokens; the nodes' own K / V rows already
+ * lie behind them, node i's in the slot of position lens[b] + i.  (A length
+ * outside [0, cap - T], or below 0 in a ring, counts as the nearest inside.)
+ * q and out: row b*T + i at q + (b*T + i) * q_ld, heads at h * head_dim.
+ * Node i sees every committed slot and the nodes j whose bit is set in mask
+ * (fgm_cuda_tree_mask's words; bits past T do not matter), or, when mask is
+ * NULL, the nodes j <= i.  window > 0: of these only the positions above
+ * pos[b*T + i] - window, a committed slot's position being its own and node
+ * j's being pos[b*T + j]; pos NULL means lens[b] + i.
+ * Per head: q8 = rint(q * (127 / max|q|)), score = (q8 . k8) * (max|q| / 127)
+ * * ks[slot] as in fgm_cuda_attend_q8; out = sum(softmax(score) * vs * v8)
+ * with the weights in f32 (attend_q8 rounds them to 16 bits, as the
+ * reference does, so the two differ by that).  A node that sees nothing gets
+ * zeros.  lse (may be NULL): log of the sum of exp(score) of row r = b*T + i,
+ * head h at lse[r * lse_row + h * lse_head]; -inf for such a node.  A query head with a value that is no
+ * finite number gives not-a-number in out and lse, in that head alone.
+ * 1 <= T <= FGM_CUDA_TREE_MAX, at most 16 query heads per KV head; ring > 0
+ * needs 0 < window and window + T - 1 <= ring; q, out 16-byte aligned, q_ld
+ * and out_ld multiples of 4. */
+int fgm_cuda_attend_tree_q8(const fgm_cuda_kv *kv, const float *q, int q_ld, int n_heads, int T,
+                            const int32_t *lens, const uint64_t *mask, const int32_t *pos,
+                            int window, float *out, int out_ld, float *lse, size_t lse_row,
+                            size_t lse_head, void *ws, size_t ws_bytes, void *stream);
+
+/* The attention weights of such a call added up per slot (kv->acc):
+ *   acc[slot] = decay * acc[slot] + sum over nodes i with take[b*T + i] != 0
+ *   (all when take is NULL) and heads h of exp(score - lse of that node and head).
+ * A slot that a node owns starts from 0, whatever it held.  lse is
+ * fgm_cuda_attend_tree_q8's for the same arguments; a node whose lse is -inf
+ * adds nothing.  The order of the sums is fixed: equal inputs give equal
+ * bits. */
+int fgm_cuda_attend_accum_q8(const fgm_cuda_kv *kv, const float *q, int q_ld, int n_heads, int T,
+                             const int32_t *lens, const uint64_t *mask, const int32_t *pos,
+                             int window, const float *lse, size_t lse_row, size_t lse_head,
+                             const uint8_t *take, float decay, void *ws, size_t ws_bytes,
+                             void *stream);
+
+/* The decode step of both: one token per sequence (T = 1, its K / V row in
+ * slot lens[b]) attends to slots [0, lens[b]] and adds its weights to
+ * kv->acc, as the two entries above would.  Linear caches (ring == 0). */
+int fgm_cuda_attend_acc_q8(const fgm_cuda_kv *kv, const float *q, int q_ld, int n_heads,
+                           const int32_t *lens, float decay, float *out, int out_ld, void *ws,
+                           size_t ws_bytes, void *stream);
+
+/* Greedy verification of drafted trees (parent as fgm_cuda_tree_mask's).
+ * token [rows][T]: the drafted tokens, target [rows][T]: the model's choice
+ * after each node.  From node 0 on, the lowest child of the last accepted
+ * node whose token is that node's target is accepted.  path [rows][T]: the
+ * accepted nodes (node 0 first), then -1; n_acc [rows]: their number;
+ * next [rows]: the target after the last one.  1 <= T <= FGM_CUDA_TREE_MAX. */
+int fgm_cuda_tree_verify(int32_t *path, int32_t *n_acc, int32_t *next, const int32_t *parent,
+                         const int32_t *token, const int32_t *target, int rows, int T,
+                         void *stream);
+
+/* Commit the accepted path in `layers` layers (kv[0 .. layers), the same rows;
+ * caps, heads and rings may differ): the rows of node path[b*T + j] move to
+ * the slot of position lens[b] + j for j < n_acc[b], with their scales and,
+ * where kv->acc / kv->tpos are set, those.  lens_new (may be NULL, not lens
+ * itself): lens[b] + n_acc[b].  path ascends with path[j] >= j, as
+ * fgm_cuda_tree_verify writes it; entries outside [j, T) are not moved. */
+int fgm_cuda_kv_accept(const fgm_cuda_kv *kv, int layers, int T, const int32_t *lens,
+                       const int32_t *path, const int32_t *n_acc, int32_t *lens_new, void *stream);
+
+/* Hold each cache to `budget` slots: of slots [0, lens[b]) keep those whose
+ * position is below sink or among the newest `recent` positions (above the
+ * largest position - recent), then those of the largest acc; equal acc keeps
+ * the lower slot, not-a-numbers rank last.  (Protected slots alone above the
+ * budget: the lowest of them.)  Kept slots below the budget stay where they
+ * are; the kept slots above it, in order, fill the evicted slots, in order,
+ * so the fewest rows move.  map [rows][budget]: the slot each slot's row came
+ * from (its own index where it stayed, -1 past a cache shorter than the
+ * budget); lens_out [rows]: min(lens, budget), may be lens.  tpos NULL: a
+ * slot's position is its index.  acc_out / tpos_out: rows of out_stride
+ * elements, or NULL: kv->acc and kv->tpos are updated in place.  Linear caches
+ * (ring == 0) of at most 524288 slots; kv->acc is needed; 1 <= budget <= cap,
+ * sink >= 0, recent >= 0. */
+int fgm_cuda_kv_evict_q8(const fgm_cuda_kv *kv, const int32_t *lens, int budget, int sink,
+                         int recent, int32_t *map, int32_t *lens_out, float *acc_out,
+                         int32_t *tpos_out, size_t out_stride, void *stream);
+
+/* fgm_cuda_qkv_post_cs for the nodes of a tree: rows b*T + i of q, k and v
+ * with rope at pos[b*T + i], the K / V rows into sequence b's cache at the
+ * slot of position lens[b] + i (and kv->tpos there, when set).  A row whose
+ * slot falls outside [0, cap) writes no cache entry. */
+int fgm_cuda_qkv_post_tree(const fgm_cuda_kv *kv, float *q, int q_ld, float *k, float *v, int kv_ld,
+                           int n_heads, int T, const float *q_norm, const float *k_norm, float eps,
+                           const float *inv_freq, const float *cs, int positions,
+                           const int32_t *pos, const int32_t *lens, void *stream);
+
 /* ------------------------------------------------------------ row argmax
  * The token choice that follows the LM head (fgm-serve/src/engine.rs:75-83,
  * :297-302): per row the first index of the largest value, NaN never

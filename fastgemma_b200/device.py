@@ -14,7 +14,10 @@ from ._lib import call
 
 
 def _s(stream):
-    return (stream or torch.cuda.current_stream()).cuda_stream
+    if stream is not None:
+        return stream.cuda_stream
+    # torch.cuda.current_stream() without its Stream object: this runs on every call
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _p(t):
@@ -273,9 +276,10 @@ def _on(stream):
 
 
 def attend_workspace(kv, n_heads, T):
-    """A workspace for the attention entries on this cache (fgm_cuda_attend_workspace)."""
+    """A workspace for the attention entries on this cache, zeroed as its first
+    use needs it; to be kept from call to call, by one stream at a time."""
     n = call("fgm_cuda_attend_workspace", C.byref(kv), n_heads, T)
-    return torch.empty(max(int(n), 1), dtype=torch.uint8, device="cuda")
+    return torch.zeros(max(int(n), 1), dtype=torch.uint8, device="cuda")
 
 
 def _ws(ws, kv, n_heads, T, stream):

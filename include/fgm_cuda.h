@@ -465,8 +465,10 @@ int fgm_cuda_tree_mask(uint64_t *mask, int32_t *pos, const int32_t *parent, cons
                        int rows, int T, void *stream);
 
 /* Bytes of workspace that the attention entries below need for this cache,
- * head count and T (any ws of at least that size, 256-byte aligned; nothing
- * in it has to be kept or cleared between calls). */
+ * head count and T.  A ws is 256-byte aligned device memory of at least that
+ * size, filled with zeros once before its first use; every call leaves it
+ * ready for the next, of any shape it is large enough for.  Calls that may
+ * overlap in time need a ws each. */
 size_t fgm_cuda_attend_workspace(const fgm_cuda_kv *kv, int n_heads, int T);
 
 /* T tokens ("nodes") of each sequence attend to its cache and to one another.

@@ -1721,8 +1721,9 @@ static int check_tree(const char *who, const fgm_cuda_kv *kv, int n_heads, int T
   if (n_heads <= 0 || n_heads % kv->kv_heads != 0 || n_heads / kv->kv_heads > 16)
     return fail(FGM_CUDA_EINVAL, "%s: heads=%d kv_heads=%d (need a multiple, at most 16 per KV head)",
                 who, n_heads, kv->kv_heads);
-  if ((long long)kv->rows * T > INT_MAX / 2)
-    return fail(FGM_CUDA_EINVAL, "%s: rows=%d T=%d", who, kv->rows, T);
+  if ((long long)kv->rows * T * n_heads > (1 << 26))
+    return fail(FGM_CUDA_EINVAL, "%s: rows=%d T=%d heads=%d (need rows * T * heads <= 2^26)", who,
+                kv->rows, T, n_heads);
   return FGM_CUDA_OK;
 }
 
@@ -1778,7 +1779,7 @@ int fgm_cuda_attend_tree_q8(const fgm_cuda_kv *kv, const float *q, int q_ld, int
   if ((rc = check_attend("attend_tree", p, ws_bytes, true)) || kv->rows == 0) return rc;
   DevInfo *di = nullptr;
   if ((rc = dev_info(&di))) return rc;
-  return glue_done(launch_attend_tree(p, di->sms, (cudaStream_t)stream), "attend_tree launch");
+  return glue_done(launch_attend_tree(p, di->sms, di->err, (cudaStream_t)stream), "attend_tree launch");
 }
 
 int fgm_cuda_attend_accum_q8(const fgm_cuda_kv *kv, const float *q, int q_ld, int n_heads, int T,

@@ -187,7 +187,10 @@ struct TreeParams {
   void *ws;
 };
 size_t attend_workspace(const fgm_cuda_kv &kv, int n_heads, int T);
-cudaError_t launch_attend_tree(const TreeParams &p, int num_sms, cudaStream_t st);
+cudaError_t launch_attend_tree(const TreeParams &p, int num_sms, int *err, cudaStream_t st);
+// kvtile.cu, more than 16 query rows per KV head; err: set when a wait gives up
+size_t attend_tile_workspace(const fgm_cuda_kv &kv, int n_heads, int T);
+cudaError_t launch_attend_tile(const TreeParams &p, int num_sms, int *err, cudaStream_t st);
 cudaError_t launch_attend_accum(const TreeParams &p, int num_sms, cudaStream_t st);
 cudaError_t launch_attend_acc(const TreeParams &p, int num_sms, cudaStream_t st);
 cudaError_t launch_tree_mask(uint64_t *mask, int32_t *pos, const int32_t *parent,
@@ -235,6 +238,9 @@ bool encode_packed_a_map(CUtensorMap *map, const void *base, int K, int rows);
 bool encode_scale_map(CUtensorMap *map, const void *base, int groups, int N, int rows);
 // .fgm int8 tiles -> row-major [N][K] (the tensor-core weight operand).
 cudaError_t launch_q8c_rows(const int8_t *tiles, int8_t *rows, int N, int K, cudaStream_t st);
+// The K rows of a cache as a 3-D TMA view (bytes of a slot, slots, sequences),
+// boxes of 128 bytes x 128 slots, 128-byte swizzle.
+bool encode_cache_map(CUtensorMap *map, const fgm_cuda_kv &kv);
 // tile-packed activations -> row-major [M][K].
 cudaError_t launch_packed_to_rows(const int8_t *packed, int8_t *rows, int M, int K,
                                   cudaStream_t st);

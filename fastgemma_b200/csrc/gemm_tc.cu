@@ -709,6 +709,20 @@ bool encode_scale_map(CUtensorMap *map, const void *base, int groups, int N, int
              CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool encode_cache_map(CUtensorMap *map, const fgm_cuda_kv &kv) {
+  auto enc = get_encode();
+  if (!enc) return false;
+  const size_t kvd = (size_t)kv.kv_heads * kv.head_dim;
+  const cuuint64_t dims[3] = {kvd, (cuuint64_t)kv.cap, (cuuint64_t)kv.rows};
+  const cuuint64_t strides[2] = {kvd, kv.rows > 1 ? kv.kc_stride : kvd * kv.cap};
+  const cuuint32_t box[3] = {128, 128, 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, kv.kc, dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 cudaError_t launch_q8c_rows(const int8_t *tiles, int8_t *rows, int N, int K, cudaStream_t st) {
   const size_t words = (size_t)N * K / 4;
   q8c_tiles_to_rows<<<grid_for(words), 256, 0, st>>>(reinterpret_cast<const uint32_t *>(tiles),

@@ -1,0 +1,250 @@
+// What the attention kernels over the KV cache share (kvattn.cu: few query
+// rows, kvtile.cu: many): visibility, the division of the work, the join of
+// partial results, launch helpers.
+#pragma once
+
+#include <atomic>
+
+#include "fgm_internal.h"
+#include "kv_common.cuh"
+
+namespace fgm {
+namespace kv {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// 2^e for -126 <= e <= 127.
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
+
+// Whether a row's node sees position t (node: -1 for a padding row).
+__device__ __forceinline__ bool sees(const TreeParams &p, int b, int node, int len, int t,
+                                     int low) {
+  if (t < 0 || node < 0) return false;
+  if (t < len) return t >= low;
+  const int j = t - len;
+  if (p.mask) {
+    const int w = (p.T + 63) / 64;
+    if (!((p.mask[((size_t)b * p.T + node) * w + (j >> 6)] >> (j & 63)) & 1)) return false;
+  } else if (j > node) {
+    return false;
+  }
+  return !p.window || (p.pos ? p.pos[b * p.T + j] : t) >= low;
+}
+
+// Slots [first, end) of sequence b that any of its nodes can see.
+struct Span {
+  int len, first, end;
+};
+__device__ __forceinline__ Span span_of(const TreeParams &p, int b) {
+  Span s;
+  s.len = committed(p.kv, p.lens, b, p.T);
+  s.end = s.len + p.T;
+  s.first = 0;
+  if (p.kv.ring) {
+    s.end = min(s.end, p.kv.ring);
+  } else if (p.window) {
+    int low = INT_MAX;
+    if (p.pos)
+      for (int i = 0; i < p.T; i++) low = min(low, lowest(p.pos[b * p.T + i], p.window));
+    else
+      low = lowest(s.len, p.window);
+    s.first = min(max(low, 0), s.len) & ~15;
+  }
+  return s;
+}
+
+// ------------------------------------------------------------- the work list
+// Items (sequence, KV head, row block) of `tiles` slot tiles each, one run of
+// an item's tiles per CTA.  Lengths are known on the device only, so every
+// warp finds its CTA's run itself: the fewest tiles per CTA (at least
+// min_per) for which all runs fit the grid, which holds at least one CTA per
+// item.  Splitting items instead of a flat list of tiles costs at most one
+// tile of balance and saves a CTA from working on two items in turn (5 us).
+constexpr int kCounters = 16384;  // grid of a launch with split items, at most
+
+struct Work {
+  int b, in_b;          // sequence, item within it
+  int t0, t1;           // tiles
+  int first, count;     // CTAs of the item
+  Span span;
+};
+
+__device__ __forceinline__ int tiles_of(const Span &s, int tile) {
+  return (s.end - s.first + tile - 1) / tile;
+}
+
+__device__ __forceinline__ bool find_work(const TreeParams &p, int tile, int per_b, int min_per,
+                                          int lane, Work &w) {
+  const int rows = p.kv.rows, grid = gridDim.x, cta = blockIdx.x;
+  const Span mine = span_of(p, min(lane, rows - 1));
+  const int n0 = lane < rows ? tiles_of(mine, tile) : 0;  // the first 32 sequences stay here
+  int total = n0;
+  for (int b = lane + 32; b < rows; b += 32) total += tiles_of(span_of(p, b), tile);
+  total = __reduce_add_sync(0xffffffffu, total);
+  const long long units = (long long)total * per_b;
+  int per = max(min_per, (int)((units + grid - 1) / grid));
+  for (;; per += 1 + per / 32) {
+    int c = (n0 + per - 1) / per;
+    for (int b = lane + 32; b < rows; b += 32)
+      c += (tiles_of(span_of(p, b), tile) + per - 1) / per;
+    if (__reduce_add_sync(0xffffffffu, c) * per_b <= grid) break;
+  }
+  int base = 0;
+  for (int b0 = 0; b0 < rows; b0 += 32) {
+    const int b = b0 + lane;
+    const Span s = b0 == 0 ? mine : span_of(p, min(b, rows - 1));
+    const int tiles = b < rows ? tiles_of(s, tile) : 0, cnt = (tiles + per - 1) / per;
+    int inc = cnt * per_b;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, base + inc > cta);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      const int t = __shfl_sync(0xffffffffu, tiles, l);
+      w.span.len = __shfl_sync(0xffffffffu, s.len, l);
+      w.span.first = __shfl_sync(0xffffffffu, s.first, l);
+      w.span.end = __shfl_sync(0xffffffffu, s.end, l);
+      w.b = b0 + l;
+      w.count = __shfl_sync(0xffffffffu, cnt, l);
+      const int rel = cta - base - __shfl_sync(0xffffffffu, inc - cnt * per_b, l);
+      w.in_b = rel / w.count;
+      const int k = rel - w.in_b * w.count, each = t / w.count, more = t - each * w.count;
+      w.first = cta - k;
+      w.t0 = k * each + min(k, more);
+      w.t1 = w.t0 + each + (k < more);
+      return true;
+    }
+    base += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  return false;
+}
+
+// What the attention kernels leave behind for an item that several CTAs work
+// on, and the join by the last of them to arrive.  counters are 0 before and
+// after every launch.
+struct Parts {
+  float *part;          // [grid][rows][hd]: sums of p vs v8
+  float2 *stat;         // [grid][rows]: maximum * log2(e), sum of p
+  int *counters;        // [first CTA of the item]
+};
+
+__device__ __forceinline__ void store_row4(const TreeParams &p, const Work &w, int kvh, int r,
+                                           int d, float4 a, float M, float L) {
+  const int hd = p.kv.head_dim, G = p.n_heads / p.kv.kv_heads, node = r / G;
+  const int h = kvh * G + r - node * G;
+  const size_t qr = (size_t)w.b * p.T + node;
+  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+  a.x *= inv, a.y *= inv, a.z *= inv, a.w *= inv;
+  *reinterpret_cast<float4 *>(p.out + qr * p.out_ld + (size_t)h * hd + d) = a;
+  if (d == 0 && p.lse)
+    p.lse[qr * p.lse_row + h * p.lse_head] = L == 0.0f ? -INFINITY : (M + log2f(L)) * kLn2;
+}
+
+// Every thread of the CTA, after its partial results are written.  sm: at
+// least rows * (count + 2) floats of shared memory that nothing else uses.
+__device__ __forceinline__ void join_parts(const TreeParams &p, const Parts &q, const Work &w,
+                                           int kvh, int row0, int rows, int ld, float *sm) {
+  __shared__ int s_last;
+  const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31;
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) {
+    s_last = atomicAdd(q.counters + w.first, 1) == w.count - 1;
+    if (s_last) q.counters[w.first] = 0;
+  }
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  const int n = w.count, hd4 = p.kv.head_dim / 4;
+  float *f = sm, *tot = sm + rows * n;
+  const float2 *stat = q.stat + (size_t)w.first * ld;
+  for (int r = tid >> 5; r < rows; r += nt >> 5) {
+    float M = -INFINITY, L = 0.0f;
+    for (int i = lane; i < n; i += 32) M = fmaxf(M, __ldcg(&stat[(size_t)i * ld + r].x));
+    M = warp_max(M);
+    const float ref = M == -INFINITY ? 0.0f : M;
+    for (int i = lane; i < n; i += 32) {
+      const float2 v = __ldcg(&stat[(size_t)i * ld + r]);
+      const float e = ex2(v.x - ref);
+      f[r * n + i] = e;
+      L += e * v.y;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    if (lane == 0) tot[2 * r] = M, tot[2 * r + 1] = L;
+  }
+  __syncthreads();
+  for (int i = tid; i < rows * hd4; i += nt) {
+    const int r = i / hd4, d = i - r * hd4;
+    const float4 *src = reinterpret_cast<const float4 *>(q.part) +
+                        ((size_t)w.first * ld + r) * hd4 + d;
+    float4 a = make_float4(0, 0, 0, 0);
+    int k = 0;
+    for (; k + 8 <= n; k += 8) {
+      float4 v[8];
+#pragma unroll
+      for (int u = 0; u < 8; u++) v[u] = __ldcg(src + (size_t)(k + u) * ld * hd4);
+#pragma unroll
+      for (int u = 0; u < 8; u++) {
+        const float e = f[r * n + k + u];
+        a.x += e * v[u].x, a.y += e * v[u].y, a.z += e * v[u].z, a.w += e * v[u].w;
+      }
+    }
+    for (; k < n; k++) {
+      const float4 v = __ldcg(src + (size_t)k * ld * hd4);
+      const float e = f[r * n + k];
+      a.x += e * v.x, a.y += e * v.y, a.z += e * v.z, a.w += e * v.w;
+    }
+    store_row4(p, w, kvh, row0 + r, d * 4, a, tot[2 * r], tot[2 * r + 1]);
+  }
+}
+
+// ------------------------------------------------------------------ host side
+inline size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// CTAs of a launch over `items`: the SMs, or, where the items are more, some
+// more than the items, so that the longer ones split.
+constexpr int kMaxSms = 256;
+inline int grid_of(const fgm_cuda_kv &kv, long long items, int tile, int num_sms) {
+  const long long most = items * ((kv.cap + tile - 1) / tile);
+  const long long want = items <= num_sms ? num_sms : items + 2 * num_sms;
+  const long long g = want <= kCounters ? want : items;
+  return (int)(most < g ? most : g);
+}
+
+// What grid_of gives at most, on any device.
+inline long long max_grid(const fgm_cuda_kv &kv, long long items, int tile) {
+  const long long most = items * ((kv.cap + tile - 1) / tile), want = items + 2 * kMaxSms;
+  return most < want ? most : want;
+}
+
+// Raises a kernel's shared-memory limit, once per device (the call is not free).
+template <class K>
+cudaError_t allow_smem(K kernel, int bytes, std::atomic<uint64_t> &done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (e != cudaSuccess || (done.load(std::memory_order_relaxed) & bit)) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
+}  // namespace kv
+}  // namespace fgm

@@ -1,0 +1,751 @@
+// Attention of many query rows per KV head over the int8 KV cache, on the
+// tcgen05 tensor cores: tiles of 128 query rows (T nodes x G heads of one KV
+// head) by 128 slots.
+//
+// Per tile: the int32 scores Q8 . K8^T (kind::i8, exact) into one of two TMEM
+// buffers; sixteen softmax warps read them (a lane a row, a quarter of the
+// tile's slots each), scale, mask and exponentiate, and write the weights p *
+// vs back over the scores as two f16 halves (22 bits together, as in the
+// streaming kernel); those are the A operand, from TMEM, of two products with
+// V (kind::f16) that add into the f32 output in TMEM.  V comes from the cache
+// as int8, four slots of a dimension per word; four warps load it and write
+// the f16 B operand (exact), 64 slots at a time.  The output is rescaled only
+// when a row's maximum has grown by more than 2^8: until then the weights just
+// grow, for which the f16 scale leaves room.
+//
+// The queries are quantised once, by a kernel before, into the swizzled blocks
+// that the tiles copy; partial results of items split over CTAs are joined by
+// one after.
+//
+// Bound by the tensor cores: a tile costs 128 * 128 * hd MACs at the int8 rate
+// and twice that at the f16 rate.  Shared memory is next: both operands of the
+// scores and V (twice) come from it, which is why V passes through registers
+// instead of being staged as int8.
+#include <type_traits>
+
+#include <cuda_fp16.h>
+
+#include "fgm_internal.h"
+#include "kv_attn.cuh"
+#include "stream_ptx.cuh"
+#include "tc_ptx.cuh"
+
+namespace fgm {
+namespace {
+
+using namespace kv;
+
+constexpr int kTM = 128;          // query rows per tile
+constexpr int kTN = 128;          // slots per tile
+constexpr int kHalf = 64;         // slots per V stage
+constexpr int kVStages = 3;
+constexpr int kSoftWarps = 16, kSoft = kSoftWarps * 32;
+constexpr int kThreads = 128 + kSoft + 128;  // loads and MMAs, softmax, V conversion
+constexpr int kQuarter = kTN / 4;  // slots of a softmax thread
+constexpr int kChunk = 128 * 128; // bytes of one 128-byte column of Q or of a K tile
+constexpr int kGrow = 8;          // log2 by which a row's maximum may grow unnoticed
+constexpr int kUnit = 5;          // f16 weights: p * vs * 2^(kUnit - ve), at most 2^(kUnit + kGrow)
+constexpr uint32_t kColS = 256;   // TMEM columns: output [0, 256), scores / weights 2 x 128
+
+struct TileParams {
+  TreeParams t;
+  int blocks, dsplit, dv;  // row blocks; CTAs that share an item's head_dim, dims of each
+  int nkb;                 // 128-byte chunks of a K row
+  int kstages;
+  const int8_t *q8;        // [rows * kv_heads * blocks][nkb][128][128]: swizzled blocks
+  const float *qs;         // their scales [..][128]
+  float *part;             // [grid][128][dv]
+  float2 *stat;            // [grid][128]
+  int2 *desc;              // [items]: first CTA, CTAs
+  int *err;
+};
+
+__device__ __forceinline__ uint64_t desc128(uint32_t a) { return tc::sdesc_sw128(a); }
+
+// D[tmem] (+)= A[tmem, f16] * B[smem desc, f16], f32 accumulate.
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// D f32, A and B f16, both K-major.
+__host__ __device__ constexpr uint32_t idesc_f16(int m, int n) {
+  return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+__device__ __forceinline__ void tmem_st_x8(uint32_t a, const uint32_t (&r)[8]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(a), "r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld_x8(uint32_t a, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+                 "=r"(r[7])
+               : "r"(a));
+}
+
+__device__ __forceinline__ void tmem_ld_x2(uint32_t a, uint32_t (&r)[2]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0,%1}, [%2];"
+               : "=r"(r[0]), "=r"(r[1])
+               : "r"(a));
+}
+
+// One row of results to global memory (bulk group of the thread).
+__device__ __forceinline__ void bulk_s2g(void *dst, const void *src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst),
+               "r"(tc::smem_u32(src)), "r"(bytes)
+               : "memory");
+}
+
+__device__ __forceinline__ void tmem_wait_st() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// Bits [a, b) of a 64-bit word, whatever a and b.
+__device__ __forceinline__ uint64_t bit_range(int a, int b) {
+  a = max(a, 0);
+  b = min(b, 64);
+  return a >= b ? 0 : (~0ull >> (64 - (b - a))) << a;
+}
+
+// Which of the positions t .. t + 31 a row sees: committed ones from `low` on,
+// nodes by its words.
+__device__ __forceinline__ uint32_t seen_from(int t, int len, int low, const uint64_t (&nodes)[4]) {
+  uint32_t v = (uint32_t)bit_range(max(low, 0) - t, len - t);
+  const int n = t - len;  // node of bit 0
+  if (n > -32 && n < FGM_CUDA_TREE_MAX) {
+    if (n < 0) {
+      v |= (uint32_t)(nodes[0] << -n);
+    } else {
+      const int w = n >> 6, s = n & 63;
+      v |= (uint32_t)(nodes[w] >> s);
+      if (w < 3 && s > 32) v |= (uint32_t)(nodes[w + 1] << (64 - s));
+    }
+  }
+  return v;
+}
+
+// int32 to f32.  |x| < 2^22 (head_dim <= 256): through the mantissa of 1.5 *
+// 2^23, on the ordinary pipes, which the conversion unit would hold up.
+__device__ __forceinline__ float dot_f32(uint32_t x, bool small) {
+  return small ? __fadd_rn(__uint_as_float(x + 0x4B400000u), -12582912.0f) : (float)(int)x;
+}
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Four int8 as two f16 pairs, exact (see the streaming kernel).
+__device__ __forceinline__ void i8x4_to_f16(uint32_t w, uint32_t &lo, uint32_t &hi) {
+  w ^= 0x80808080u;
+  const __half2 off = __floats2half2_rn(1152.0f, 1152.0f);
+  uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+  const __half2 x = __hsub2(*reinterpret_cast<__half2 *>(&a), off);
+  const __half2 y = __hsub2(*reinterpret_cast<__half2 *>(&b), off);
+  lo = *reinterpret_cast<const uint32_t *>(&x);
+  hi = *reinterpret_cast<const uint32_t *>(&y);
+}
+
+struct Bars {
+  uint64_t q_full, k_full[4], k_empty[4], v_full[kVStages], v_empty[kVStages], s_full[2], p_full[2],
+      sc_full[2], pv_done;
+};
+
+__global__ void __launch_bounds__(kThreads, 1)
+    tile_kernel(const __grid_constant__ TileParams tp, const __grid_constant__ CUtensorMap kmap) {
+  extern __shared__ uint8_t raw[];
+  __shared__ __align__(8) Bars bar;
+  __shared__ __align__(16) float s_ks[2][kTN], s_vs[2][kTN];
+  __shared__ float s_max[2][4][kTM], s_l[4][kTM];
+  __shared__ int s_pos[FGM_CUDA_TREE_MAX], s_low[kTM];
+  __shared__ uint64_t s_see[kTM][4];  // nodes each row sees
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort, s_ve;
+  const TreeParams &p = tp.t;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int hd = p.kv.head_dim, kvd = p.kv.kv_heads * hd, G = p.n_heads / p.kv.kv_heads;
+  const int R = p.T * G, dv = tp.dv;
+  uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t *q8 = sm, *ksm = q8 + tp.nkb * kChunk, *vf = ksm + tp.kstages * kChunk;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  Work wk;
+  if (!find_work(p, kTN, p.kv.kv_heads * tp.blocks * tp.dsplit, 1, lane, wk)) return;
+  const int b = wk.b, ds = wk.in_b % tp.dsplit, blk = wk.in_b / tp.dsplit % tp.blocks;
+  const int kvh = wk.in_b / (tp.dsplit * tp.blocks), row0 = blk * kTM, rows = min(kTM, R - row0);
+  const int len = wk.span.len, ring = p.kv.ring, end = len + p.T;
+  const int x0 = wk.span.first + wk.t0 * kTN, x1 = min(wk.span.end, wk.span.first + wk.t1 * kTN);
+  const int tiles = wk.t1 - wk.t0;
+  const float *ks = p.kv.ks + (size_t)b * p.kv.ks_stride;
+  const float *vs = p.kv.vs + (size_t)b * p.kv.vs_stride;
+
+  if (tid == 0) {
+    for (int i = 0; i < 4; i++) {
+      tc::mbar_init(&bar.k_full[i], 1);
+      tc::mbar_init(&bar.k_empty[i], 1);
+    }
+    for (int i = 0; i < kVStages; i++) {
+      tc::mbar_init(&bar.v_full[i], 128);
+      tc::mbar_init(&bar.v_empty[i], 1);
+    }
+    for (int i = 0; i < 2; i++) {
+      tc::mbar_init(&bar.s_full[i], 1);
+      tc::mbar_init(&bar.p_full[i], kSoft);
+      tc::mbar_init(&bar.sc_full[i], 32);
+    }
+    tc::mbar_init(&bar.q_full, 1);
+    tc::mbar_init(&bar.pv_done, 1);
+    tc::fence_mbar_init();
+    s_abort = 0;
+    s_ve = -100;
+    tc::prefetch_tmap(&kmap);
+    if (wk.t0 == 0) tp.desc[b * p.kv.kv_heads * tp.blocks * tp.dsplit + wk.in_b] =
+        make_int2(wk.first, wk.count);
+  }
+  if (warp == 1) {
+    tc::tmem_alloc(&s_tmem, 512);
+    tc::tmem_relinquish();
+  }
+  __syncthreads();
+
+  // A wait that gives up raises the abort word; from then on every wait
+  // returns at once, the loops run out and the CTA leaves.
+  auto wait = [&](uint64_t *w, uint32_t parity) {
+    if (tc::mbar_try_wait(w, parity) || *(volatile int *)&s_abort) return;
+    if (!tc::mbar_wait(w, parity)) {
+      *(volatile int *)&s_abort = 1;
+      if (tp.err) atomicExch(tp.err, 1);
+    }
+  };
+
+  // first K and V stages on their way (their barriers are fresh)
+  auto load_k = [&](int c) {  // chunk c: tile c / nkb, bytes 128 * (c % nkb) of the rows
+    const int st = c % tp.kstages, t = c / tp.nkb;
+    tc::mbar_expect_tx(&bar.k_full[st], kChunk);
+    tc::tma_load_3d(ksm + st * kChunk, &kmap, &bar.k_full[st],
+                    kvh * hd + (c - t * tp.nkb) * 128, x0 + t * kTN, b);
+  };
+  const int chunks = tiles * tp.nkb, halves = tiles * 2;
+  if (warp == 0 && lane == 0)
+    for (int c = 0; c < min(chunks, tp.kstages); c++) load_k(c);
+
+  // the largest |vs| of the run: the unit of the f16 weights
+  auto exponent = [&](int x) {
+    if (x >= x1 || pos_of(ring, x, end) < 0) return -100;
+    const float v = fabsf(vs[x]);
+    if (!(v > 0.0f && v < INFINITY)) return -100;
+    return max(-100, min((int)((__float_as_uint(v) >> 23) & 255) - 126, 126));
+  };
+  int top_e = -100;
+  for (int x = x0 + tid; x < x1; x += kThreads) top_e = max(top_e, exponent(x));
+  top_e = __reduce_max_sync(0xffffffffu, top_e);
+  if (lane == 0) atomicMax(&s_ve, top_e);
+  if (tid < kTM) {
+    const int node = (row0 + tid) / G;
+    s_low[tid] = tid < rows ? lowest(p.pos ? p.pos[b * p.T + node] : len + node, p.window) : INT_MIN;
+  }
+  if (p.window)
+    for (int i = tid; i < p.T; i += kThreads) s_pos[i] = p.pos ? p.pos[b * p.T + i] : len + i;
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = s_tmem;
+  const size_t qblock = ((size_t)b * p.kv.kv_heads + kvh) * tp.blocks + blk;
+
+  if (warp == 0) {  // ---- the queries, K chunks
+    if (lane == 0) {
+      stream::pdl_wait();  // for the kernel that quantised the queries
+      tc::mbar_expect_tx(&bar.q_full, (uint32_t)tp.nkb * kChunk);
+      stream::bulk_g2s(tc::smem_u32(q8), tp.q8 + qblock * tp.nkb * kChunk,
+                       (uint32_t)tp.nkb * kChunk, &bar.q_full);
+      for (int c = tp.kstages; c < chunks; c++) {
+        const int st = c % tp.kstages;
+        wait(&bar.k_empty[st], (c / tp.kstages - 1) & 1);
+        load_k(c);
+      }
+    }
+  } else if (warp == 2) {  // ---- scales of the slots, two tiles ahead
+    const float unit = pow2(kUnit - s_ve);
+    for (int j = 0; j < tiles; j++) {
+      float a[4], c[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const int x = x0 + j * kTN + lane + 32 * k;
+        a[k] = x < x1 ? ks[x] : 0.0f;
+        c[k] = x < x1 ? vs[x] * unit : 0.0f;
+      }
+      if (j >= 2) wait(&bar.p_full[j & 1], ((j - 2) >> 1) & 1);
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        s_ks[j & 1][lane + 32 * k] = a[k];
+        s_vs[j & 1][lane + 32 * k] = c[k];
+      }
+      tc::mbar_arrive(&bar.sc_full[j & 1]);
+    }
+  } else if (warp == 1) {  // ---- MMAs
+    if (lane == 0) {
+      // descriptors differ from these in their address field, 16 bytes a unit
+      const uint64_t qd = desc128(tc::smem_u32(q8)), kd = desc128(tc::smem_u32(ksm));
+      const uint64_t vd = desc128(tc::smem_u32(vf));
+      const uint32_t id_s = tc::idesc_i8(kTM, kTN), id_o = idesc_f16(kTM, dv);
+      int kst = 0, vst = 0;
+      uint32_t kph = 0, vph = 0;
+      auto scores = [&](int j) {
+        const uint32_t d = tmem + kColS + (j & 1) * kTN;
+        for (int kb = 0; kb < tp.nkb; kb++) {
+          wait(&bar.k_full[kst], kph);
+          tc::fence_after_sync();
+          const uint64_t a = qd + kb * (kChunk >> 4), c = kd + kst * (kChunk >> 4);
+          tc::mma_i8(d, a, c, id_s, kb > 0);
+          tc::mma_i8(d, a + 2, c + 2, id_s, 1);
+          if (hd - kb * 128 >= 128) {
+            tc::mma_i8(d, a + 4, c + 4, id_s, 1);
+            tc::mma_i8(d, a + 6, c + 6, id_s, 1);
+          }
+          tc::mma_commit(&bar.k_empty[kst]);
+          if (++kst == tp.kstages) kst = 0, kph ^= 1;
+        }
+        tc::mma_commit(&bar.s_full[j & 1]);
+      };
+      wait(&bar.q_full, 0);
+      scores(0);
+      if (tiles > 1) scores(1);
+      for (int j = 0; j < tiles; j++) {
+        const uint32_t pb = tmem + kColS + (j & 1) * kTN;
+        wait(&bar.p_full[j & 1], (j >> 1) & 1);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          wait(&bar.v_full[vst], vph);
+          tc::fence_after_sync();
+          const uint64_t v = vd + vst * (dv * 8);
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            mma_f16_ts(tmem, pb + (h * 4 + k) * 8, v + k * 2, id_o, j + h + k > 0);
+            mma_f16_ts(tmem, pb + 64 + (h * 4 + k) * 8, v + k * 2, id_o, 1);
+          }
+          tc::mma_commit(&bar.v_empty[vst]);
+          if (++vst == kVStages) vst = 0, vph ^= 1;
+        }
+        tc::mma_commit(&bar.pv_done);
+        if (j + 2 < tiles) {  // the weights' columns take new scores once they are read
+          wait(&bar.pv_done, j & 1);
+          scores(j + 2);
+        }
+      }
+    }
+  } else if (warp >= 4 + kSoftWarps) {  // ---- V to f16, K-major: a row per dimension, 64 slots
+    // A thread takes four dimensions of two slot groups at a time: dimension
+    // 4 i + e becomes row e * dv / 4 + i, so that a warp's rows follow one
+    // another and its stores meet no bank twice.  Loads run half a tile ahead.
+    const int t = tid - (4 + kSoftWarps) * 32, quads = dv / 4;
+    const uint8_t *src = reinterpret_cast<const uint8_t *>(p.kv.vt) + (size_t)b * p.kv.vt_stride +
+                         (size_t)(kvh * hd + ds * dv) * 4;
+    const int gend = (x1 + 3) >> 2;
+    uint4 w[4][2];
+    auto load = [&](int h) {
+      const int g0 = (x0 + h * kHalf) >> 2;
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const int i = t + 128 * k, pair = i / quads, q = i - pair * quads, g = g0 + 2 * pair;
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+          w[k][e] = pair < 8 && g + e < gend
+                        ? __ldg(reinterpret_cast<const uint4 *>(src + (size_t)(g + e) * kvd * 4) + q)
+                        : make_uint4(0, 0, 0, 0);
+      }
+    };
+    load(0);
+    int st = 0;
+    uint32_t ph = 1;  // the parity of the stage's last release; fresh stages are free
+    for (int h = 0; h < halves; h++) {
+      if (h >= kVStages) wait(&bar.v_empty[st], ph);
+      uint8_t *dst = vf + st * (dv * 128);
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const int i = t + 128 * k, pair = i / quads, q = i - pair * quads;
+        const uint32_t a[4] = {w[k][0].x, w[k][0].y, w[k][0].z, w[k][0].w};
+        const uint32_t c[4] = {w[k][1].x, w[k][1].y, w[k][1].z, w[k][1].w};
+        if (pair < 8)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const int r = e * quads + q;
+            uint4 o;
+            i8x4_to_f16(a[e], o.x, o.y);
+            i8x4_to_f16(c[e], o.z, o.w);
+            *reinterpret_cast<uint4 *>(dst + r * 128 + ((pair ^ (r & 7)) << 4)) = o;
+          }
+      }
+      if (h + 1 < halves) load(h + 1);
+      stream::fence_proxy_async_smem();
+      tc::mbar_arrive(&bar.v_full[st]);
+      if (++st == kVStages) st = 0, ph ^= 1;
+    }
+  } else if (warp >= 4) {  // ---- softmax: row (warp % 4) * 32 + lane, slots 32 * quarter ...
+    const int quarter = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t quad = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const int r = row0 + row, node = row < rows ? r / G : -1, low = s_low[row];
+    const bool idle = (warp & 3) * 32 >= rows;  // only padding rows: nothing to compute
+    stream::pdl_wait();
+    const float qs = row < rows ? tp.qs[qblock * kTM + row] : 1e-37f;
+    const int high = __reduce_max_sync(
+        0xffffffffu, max(max(s_low[lane], s_low[lane + 32]), max(s_low[lane + 64], s_low[lane + 96])));
+    {  // the nodes this row sees, a word per quarter
+      uint64_t v = 0;
+      const int w = quarter;
+      if (node >= 0 && w * 64 < p.T) {
+        v = p.mask ? p.mask[((size_t)b * p.T + node) * ((p.T + 63) / 64) + w]
+                   : bit_range(0, node + 1 - w * 64);
+        v &= bit_range(0, p.T - w * 64);
+        if (p.window)
+          for (int i = 0; i < min(64, p.T - w * 64); i++)
+            if (s_pos[w * 64 + i] < low) v &= ~(1ull << i);
+      }
+      s_see[row][w] = v;
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory");
+    // position of slot x: x + (x <= turn ? lo_off : hi_off)
+    const int turn = ring ? (end - 1) % ring : INT_MAX;
+    const int lo_off = ring ? end - 1 - turn : 0, hi_off = lo_off - ring;
+    const bool small = hd <= 256;
+    float m = -INFINITY, l = 0.0f;
+
+    auto tile = [&](int j, auto is_masked) {
+      constexpr bool masked = decltype(is_masked)::value;
+      const int buf = j & 1;
+      const uint32_t sc = quad + kColS + buf * kTN;
+      const float *ksq = s_ks[buf] + quarter * kQuarter, *vsq = s_vs[buf] + quarter * kQuarter;
+      uint32_t s[kQuarter];
+      tc::tmem_ld_x32(sc + quarter * kQuarter, s);
+      uint32_t seen = 0;
+      if (masked) {
+        const int x = x0 + j * kTN + quarter * kQuarter, cut = turn - x;
+        seen = seen_from(x + (cut >= 0 ? lo_off : hi_off), len, low, s_see[row]);
+        if (cut >= 0 && cut < kQuarter - 1) {  // the ring turns inside these slots
+          const uint32_t before = (2u << cut) - 1;
+          seen = (seen & before) | (seen_from(x + hi_off, len, low, s_see[row]) & ~before);
+        }
+        seen &= (uint32_t)bit_range(0, x1 - x);
+        if (node < 0) seen = 0;
+      }
+      tc::tmem_wait_ld();
+      float top = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < kQuarter; c += 4) {
+        const float4 k4 = *reinterpret_cast<const float4 *>(ksq + c);
+        float u[4] = {dot_f32(s[c], small) * k4.x, dot_f32(s[c + 1], small) * k4.y,
+                      dot_f32(s[c + 2], small) * k4.z, dot_f32(s[c + 3], small) * k4.w};
+        if (masked)
+#pragma unroll
+          for (int k = 0; k < 4; k++)
+            if (!((seen >> (c + k)) & 1)) u[k] = -INFINITY;
+        top = fmaxf(fmaxf(top, fmaxf(u[0], u[1])), fmaxf(u[2], u[3]));
+#pragma unroll
+        for (int k = 0; k < 4; k++) s[c + k] = __float_as_uint(u[k]);
+      }
+      s_max[buf][quarter][row] = top;
+      asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory");
+      top = fmaxf(fmaxf(s_max[buf][0][row], s_max[buf][1][row]),
+                  fmaxf(s_max[buf][2][row], s_max[buf][3][row])) * qs;
+      // a growing maximum: the sum and, once something was added, the output
+      float f = 1.0f;
+      if (top > m + kGrow || m == -INFINITY) {
+        f = m == -INFINITY ? 1.0f : ex2(m - top);
+        m = top;
+        l *= f;
+      }
+      if (__any_sync(0xffffffffu, f != 1.0f)) {
+        wait(&bar.pv_done, (j - 1) & 1);
+        tc::fence_after_sync();
+        for (int c = quarter * (dv / 4); c < (quarter + 1) * (dv / 4); c += 8) {
+          uint32_t o[8];
+          tmem_ld_x8(quad + c, o);
+          tc::tmem_wait_ld();
+#pragma unroll
+          for (int k = 0; k < 8; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+          tmem_st_x8(quad + c, o);
+        }
+        tmem_wait_st();
+      }
+      const float ref = m == -INFINITY ? 0.0f : m;
+      float la = 0.0f, lb = 0.0f;
+#pragma unroll
+      for (int c0 = 0; c0 < kQuarter; c0 += 16) {
+        uint32_t hi[8], lo[8];
+#pragma unroll
+        for (int c = 0; c < 16; c += 4) {
+          const float4 v4 = *reinterpret_cast<const float4 *>(vsq + c0 + c);
+          const float vv[4] = {v4.x, v4.y, v4.z, v4.w};
+          float w[4];
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            const float e = ex2(__fmaf_rn(__uint_as_float(s[c0 + c + k]), qs, -ref));
+            if (k & 1) lb += e;
+            else la += e;
+            w[k] = e * vv[k];
+            // an unseen slot's scale may be anything
+            if (masked && !((seen >> (c0 + c + k)) & 1)) w[k] = 0.0f;
+          }
+#pragma unroll
+          for (int k = 0; k < 4; k += 2) {
+            const __half2 h2 = __floats2half2_rn(w[k], w[k + 1]);
+            const float2 hf = __half22float2(h2);
+            hi[(c + k) / 2] = *reinterpret_cast<const uint32_t *>(&h2);
+            lo[(c + k) / 2] = pack2(w[k] - hf.x, w[k + 1] - hf.y);
+          }
+        }
+        tmem_st_x8(sc + quarter * 16 + c0 / 2, hi);
+        tmem_st_x8(sc + 64 + quarter * 16 + c0 / 2, lo);
+      }
+      l += la + lb;
+      tmem_wait_st();
+    };
+    for (int j = 0; j < tiles; j++) {
+      wait(&bar.sc_full[j & 1], (j >> 1) & 1);
+      wait(&bar.s_full[j & 1], (j >> 1) & 1);
+      tc::fence_after_sync();
+      if (idle) asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory");
+      else if (ring || x0 + (j + 1) * kTN > len || x0 + j * kTN < high)
+        tile(j, std::true_type());
+      else
+        tile(j, std::false_type());
+      tc::fence_before_sync();
+      tc::mbar_arrive(&bar.p_full[j & 1]);
+    }
+    // ---- results: the quarters' sums joined, each quarter's dimensions to
+    // shared memory, whole rows from there (what the loads filled is free now)
+    s_l[quarter][row] = l;
+    asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory");
+    const float L = (s_l[0][row] + s_l[1][row]) + (s_l[2][row] + s_l[3][row]);
+    wait(&bar.pv_done, (tiles - 1) & 1);
+    tc::fence_after_sync();
+    const bool whole = wk.count == 1;
+    float back = pow2(s_ve) * 0.03125f;  // 2^-kUnit
+    if (whole) back = L == 0.0f ? 0.0f : back / L;
+    float *stage = reinterpret_cast<float *>(sm + (size_t)row * (dv * 4 + 16));
+    if (!idle)  // column e * dv / 4 + i of the output is dimension 4 i + e
+#pragma unroll 4
+      for (int i = quarter * (dv / 16); i < (quarter + 1) * (dv / 16); i += 2) {
+        uint32_t o[4][2];
+#pragma unroll
+        for (int e = 0; e < 4; e++) tmem_ld_x2(quad + e * (dv / 4) + i, o[e]);
+        tc::tmem_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+          *reinterpret_cast<float4 *>(stage + 4 * (i + k)) =
+              make_float4(__uint_as_float(o[0][k]) * back, __uint_as_float(o[1][k]) * back,
+                          __uint_as_float(o[2][k]) * back, __uint_as_float(o[3][k]) * back);
+      }
+    tc::fence_before_sync();
+    stream::fence_proxy_async_smem();
+    asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory");
+    if (quarter == 0 && row < rows) {
+      const int h = kvh * G + r - node * G;
+      const size_t qr = (size_t)b * p.T + node;
+      bulk_s2g(whole ? p.out + qr * p.out_ld + (size_t)h * hd + ds * dv
+                     : tp.part + ((size_t)blockIdx.x * kTM + row) * dv, stage, (uint32_t)dv * 4);
+      tc::bulk_commit();
+      if (!whole) tp.stat[(size_t)blockIdx.x * kTM + row] = make_float2(m, L);
+      else if (ds == 0 && p.lse)
+        p.lse[qr * p.lse_row + h * p.lse_head] = L == 0.0f ? -INFINITY : (m + log2f(L)) * kLn2;
+      tc::bulk_wait_all();
+    }
+  }
+  __syncthreads();
+  if (s_abort) {  // copies that nobody waited for still land in shared memory
+    if (warp == 0 && lane == 0)
+      for (int c = max(0, chunks - tp.kstages); c < chunks; c++)
+        tc::mbar_wait(&bar.k_full[c % tp.kstages], (c / tp.kstages) & 1);
+    if (warp == 0 && lane == 0) tc::mbar_wait(&bar.q_full, 0);
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc::fence_after_sync();
+    tc::tmem_dealloc(tmem, 512);
+  }
+}
+
+// A warp per query row: its int8 copy in the block's swizzled place, its scale
+// times log2(e).
+constexpr int kQuantRows = 8;
+__global__ void __launch_bounds__(kQuantRows * 32)
+    quant_rows_kernel(const __grid_constant__ TreeParams p, int blocks, int nkb, int8_t *q8,
+                      float *qs) {
+  const int lane = threadIdx.x & 31, row = blockIdx.x * kQuantRows + (threadIdx.x >> 5);
+  const int hd = p.kv.head_dim, G = p.n_heads / p.kv.kv_heads, R = p.T * G;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int bk = row / R, r = row - bk * R, b = bk / p.kv.kv_heads, kvh = bk - b * p.kv.kv_heads;
+  if (b >= p.kv.rows) return;
+  const int node = r / G;
+  const float4 *src = reinterpret_cast<const float4 *>(
+      p.q + ((size_t)b * p.T + node) * p.q_ld + (size_t)(kvh * G + r - node * G) * hd);
+  float4 v[4];
+  float top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    v[i] = lane + 32 * i < hd / 4 ? src[lane + 32 * i] : make_float4(0, 0, 0, 0);
+    top = fmaxf(fmaxf(top, fmaxf(q_abs(v[i].x), q_abs(v[i].y))),
+                fmaxf(q_abs(v[i].z), q_abs(v[i].w)));
+  }
+  top = warp_max(top);
+  const float inv = q_inv(top);
+  const size_t block = (size_t)bk * blocks + r / kTM;
+  const int j = r % kTM;
+  int8_t *dst = q8 + block * nkb * kChunk + j * 128 + (((lane >> 2) ^ (j & 7)) << 4) + (lane & 3) * 4;
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    if (lane + 32 * i < hd / 4)
+      *reinterpret_cast<uint32_t *>(dst + i * kChunk) =
+          (q_int8(v[i].x, inv) & 255) | (q_int8(v[i].y, inv) & 255) << 8 |
+          (q_int8(v[i].z, inv) & 255) << 16 | q_int8(v[i].w, inv) << 24;
+  // never 0, so that a masked score stays -inf (a zero query's dots are 0)
+  if (lane == 0)
+    qs[block * kTM + j] =
+        fmaxf(q_scale(top) * kLog2e, 1e-37f) + (top < INFINITY ? 0.0f : q_scale(top));
+}
+
+// Joins an item's partial results: a CTA takes a few rows, a thread four
+// dimensions of one.  The first parts' values are asked for together with
+// their statistics.
+constexpr int kJoin = 256;
+__global__ void __launch_bounds__(kJoin) tile_join_kernel(const __grid_constant__ TileParams tp,
+                                                          int groups) {
+  const TreeParams &p = tp.t;
+  const int hd = p.kv.head_dim, G = p.n_heads / p.kv.kv_heads, R = p.T * G, dv = tp.dv, dv4 = dv / 4;
+  const int item = blockIdx.x / groups, per_row = kJoin / dv4;
+  const int in_row = threadIdx.x / dv4, d = threadIdx.x - in_row * dv4;
+  const int row = (blockIdx.x - item * groups) * per_row + in_row;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int per_b = p.kv.kv_heads * tp.blocks * tp.dsplit;
+  const int b = item / per_b, in_b = item - b * per_b;
+  const int ds = in_b % tp.dsplit, blk = in_b / tp.dsplit % tp.blocks;
+  const int kvh = in_b / (tp.dsplit * tp.blocks), r = blk * kTM + row;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (in_row >= per_row || row >= kTM || r >= R) return;
+  const int2 de = tp.desc[item];
+  if (de.y == 1) return;
+  const float2 *stat = tp.stat + (size_t)de.x * kTM + row;
+  const float4 *part = reinterpret_cast<const float4 *>(tp.part) + ((size_t)de.x * kTM + row) * dv4 + d;
+  float M = -INFINITY, L = 0.0f;
+  float4 a = make_float4(0, 0, 0, 0);
+  for (int i0 = 0; i0 < de.y; i0 += 8) {
+    float2 s[8];
+    float4 v[8];
+    const int n = min(8, de.y - i0);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      s[i] = i < n ? stat[(size_t)(i0 + i) * kTM] : make_float2(-INFINITY, 0.0f);
+      v[i] = i < n ? part[(size_t)(i0 + i) * kTM * dv4] : make_float4(0, 0, 0, 0);
+    }
+    float N = M;
+#pragma unroll
+    for (int i = 0; i < 8; i++) N = fmaxf(N, s[i].x);
+    const float ref = N == -INFINITY ? 0.0f : N, f0 = ex2(M - ref);
+    a.x *= f0, a.y *= f0, a.z *= f0, a.w *= f0;
+    L *= f0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const float f = ex2(s[i].x - ref);
+      L += f * s[i].y;
+      a.x += f * v[i].x, a.y += f * v[i].y, a.z += f * v[i].z, a.w += f * v[i].w;
+    }
+    M = N;
+  }
+  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+  const int node = r / G, h = kvh * G + r - node * G;
+  const size_t qr = (size_t)b * p.T + node;
+  reinterpret_cast<float4 *>(p.out + qr * p.out_ld + (size_t)h * hd + ds * dv)[d] =
+      make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+  if (d == 0 && ds == 0 && p.lse)
+    p.lse[qr * p.lse_row + h * p.lse_head] = L == 0.0f ? -INFINITY : (M + log2f(L)) * kLn2;
+}
+
+constexpr int kMaxSmem = 210 * 1024;  // of any head_dim
+
+struct TilePlan {
+  int blocks, dsplit, dv, nkb, kstages;
+  long long items;
+  size_t smem, part, stat, desc, q8, qs, total;
+};
+
+TilePlan tile_plan(const fgm_cuda_kv &kv, int n_heads, int T) {
+  TilePlan q;
+  const int hd = kv.head_dim, R = T * (n_heads / kv.kv_heads);
+  q.blocks = (R + kTM - 1) / kTM;
+  q.dsplit = hd > 256 ? 2 : 1;
+  q.dv = hd / q.dsplit;
+  q.nkb = (hd + 127) / 128;
+  q.kstages = q.nkb > 2 ? 3 : 4;
+  q.items = (long long)kv.rows * kv.kv_heads * q.blocks * q.dsplit;
+  q.smem = 1024 + (size_t)(q.nkb + q.kstages) * kChunk + (size_t)kVStages * q.dv * 128;
+  const size_t grid = (size_t)max_grid(kv, q.items, kTN);
+  q.part = kCounters * sizeof(int);
+  q.stat = q.part + align256(grid * kTM * q.dv * sizeof(float));
+  q.desc = q.stat + align256(grid * kTM * sizeof(float2));
+  q.q8 = q.desc + align256((size_t)q.items * sizeof(int2));
+  const size_t qblocks = (size_t)kv.rows * kv.kv_heads * q.blocks;
+  q.qs = q.q8 + qblocks * q.nkb * kChunk;
+  q.total = q.qs + align256(qblocks * kTM * sizeof(float));
+  return q;
+}
+
+}  // namespace
+
+size_t attend_tile_workspace(const fgm_cuda_kv &kv, int n_heads, int T) {
+  return tile_plan(kv, n_heads, T).total;
+}
+
+cudaError_t launch_attend_tile(const TreeParams &p, int num_sms, int *err, cudaStream_t st) {
+  const TilePlan q = tile_plan(p.kv, p.n_heads, p.T);
+  uint8_t *ws = static_cast<uint8_t *>(p.ws);
+  TileParams tp;
+  tp.t = p;
+  tp.blocks = q.blocks;
+  tp.dsplit = q.dsplit;
+  tp.dv = q.dv;
+  tp.nkb = q.nkb;
+  tp.kstages = q.kstages;
+  tp.q8 = reinterpret_cast<const int8_t *>(ws + q.q8);
+  tp.qs = reinterpret_cast<const float *>(ws + q.qs);
+  tp.part = reinterpret_cast<float *>(ws + q.part);
+  tp.stat = reinterpret_cast<float2 *>(ws + q.stat);
+  tp.desc = reinterpret_cast<int2 *>(ws + q.desc);
+  tp.err = err;
+  CUtensorMap kmap;
+  if (!encode_cache_map(&kmap, p.kv)) return cudaErrorInvalidValue;
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = allow_smem(tile_kernel, kMaxSmem, done);
+  if (e != cudaSuccess) return e;
+  const int R = p.T * (p.n_heads / p.kv.kv_heads), rows = R < kTM ? R : kTM;
+  const long long all = (long long)p.kv.rows * p.kv.kv_heads * R;
+  quant_rows_kernel<<<(unsigned)((all + kQuantRows - 1) / kQuantRows), kQuantRows * 32, 0, st>>>(
+      p, q.blocks, q.nkb, reinterpret_cast<int8_t *>(ws + q.q8),
+      reinterpret_cast<float *>(ws + q.qs));
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cfg.stream = st;
+  cfg.gridDim = dim3((unsigned)grid_of(p.kv, q.items, kTN, num_sms));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = q.smem;
+  if ((e = cudaLaunchKernelEx(&cfg, tile_kernel, tp, kmap)) != cudaSuccess) return e;
+  const int per = kJoin / (q.dv / 4), groups = (rows + per - 1) / per;
+  cfg.gridDim = dim3((unsigned)(q.items * groups));
+  cfg.blockDim = dim3(kJoin);
+  cfg.dynamicSmemBytes = 0;
+  return cudaLaunchKernelEx(&cfg, tile_join_kernel, tp, groups);
+}
+
+}  // namespace fgm

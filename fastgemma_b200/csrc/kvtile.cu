@@ -133,10 +133,29 @@ __device__ __forceinline__ uint32_t seen_from(int t, int len, int low, const uin
   return v;
 }
 
-// int32 to f32.  |x| < 2^22 (head_dim <= 256): through the mantissa of 1.5 *
-// 2^23, on the ordinary pipes, which the conversion unit would hold up.
-__device__ __forceinline__ float dot_f32(uint32_t x, bool small) {
-  return small ? __fadd_rn(__uint_as_float(x + 0x4B400000u), -12582912.0f) : (float)(int)x;
+// Two f32 in one register pair: the packed forms of the FP32 pipe.
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ void split2(uint64_t d, float &a, float &b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(d));
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
 }
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -155,11 +174,27 @@ __device__ __forceinline__ void i8x4_to_f16(uint32_t w, uint32_t &lo, uint32_t &
   hi = *reinterpret_cast<const uint32_t *>(&y);
 }
 
+// mbarrier test that may put the warp to sleep for up to 10 us: what waits for
+// long should not take issue slots from what works.
+__device__ __forceinline__ bool mbar_sleep(uint64_t *bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(tc::smem_u32(bar)), "r"(parity), "r"(10000u)
+      : "memory");
+  return ok != 0;
+}
+
 struct Bars {
   uint64_t q_full, k_full[4], k_empty[4], v_full[kVStages], v_empty[kVStages], s_full[2], p_full[2],
       sc_full[2], pv_done;
 };
 
+// SMALL: head_dim <= 256, so that |q8 . k8| < 2^22.
+template <bool SMALL>
 __global__ void __launch_bounds__(kThreads, 1)
     tile_kernel(const __grid_constant__ TileParams tp, const __grid_constant__ CUtensorMap kmap) {
   extern __shared__ uint8_t raw[];
@@ -220,14 +255,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   // A wait that gives up raises the abort word; from then on every wait
   // returns at once, the loops run out and the CTA leaves.
   auto wait = [&](uint64_t *w, uint32_t parity) {
-    if (tc::mbar_try_wait(w, parity) || *(volatile int *)&s_abort) return;
-    if (!tc::mbar_wait(w, parity)) {
-      *(volatile int *)&s_abort = 1;
-      if (tp.err) atomicExch(tp.err, 1);
+    if (tc::mbar_try_wait(w, parity)) return;
+    const uint64_t t0 = tc::globaltimer_ns();
+    while (!mbar_sleep(w, parity)) {
+      if (*(volatile int *)&s_abort) return;
+      if (tc::globaltimer_ns() - t0 > 2000000000ull) {
+        *(volatile int *)&s_abort = 1;
+        if (tp.err) atomicExch(tp.err, 1);
+        return;
+      }
     }
   };
 
-  // first K and V stages on their way (their barriers are fresh)
+  // first K stages on their way (their barriers are fresh)
   auto load_k = [&](int c) {  // chunk c: tile c / nkb, bytes 128 * (c % nkb) of the rows
     const int st = c % tp.kstages, t = c / tp.nkb;
     tc::mbar_expect_tx(&bar.k_full[st], kChunk);
@@ -351,17 +391,25 @@ __global__ void __launch_bounds__(kThreads, 1)
                          (size_t)(kvh * hd + ds * dv) * 4;
     const int gend = (x1 + 3) >> 2;
     uint4 w[4][2];
+    uint32_t to[4];  // where a unit's first row goes; rows are quads apart
+    int pairs[4], from[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const int i = t + 128 * k, q = i % quads;
+      pairs[k] = i / quads;
+      from[k] = 2 * pairs[k] * kvd * 4 + q * 16;
+      to[k] = q * 128 + ((pairs[k] ^ (q & 7)) << 4);  // quads is a multiple of 8
+    }
     auto load = [&](int h) {
       const int g0 = (x0 + h * kHalf) >> 2;
+      const uint8_t *base = src + (size_t)g0 * kvd * 4;
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const int i = t + 128 * k, pair = i / quads, q = i - pair * quads, g = g0 + 2 * pair;
+      for (int k = 0; k < 4; k++)
 #pragma unroll
         for (int e = 0; e < 2; e++)
-          w[k][e] = pair < 8 && g + e < gend
-                        ? __ldg(reinterpret_cast<const uint4 *>(src + (size_t)(g + e) * kvd * 4) + q)
+          w[k][e] = pairs[k] < 8 && g0 + 2 * pairs[k] + e < gend
+                        ? __ldg(reinterpret_cast<const uint4 *>(base + from[k] + e * kvd * 4))
                         : make_uint4(0, 0, 0, 0);
-      }
     };
     load(0);
     int st = 0;
@@ -371,17 +419,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint8_t *dst = vf + st * (dv * 128);
 #pragma unroll
       for (int k = 0; k < 4; k++) {
-        const int i = t + 128 * k, pair = i / quads, q = i - pair * quads;
         const uint32_t a[4] = {w[k][0].x, w[k][0].y, w[k][0].z, w[k][0].w};
         const uint32_t c[4] = {w[k][1].x, w[k][1].y, w[k][1].z, w[k][1].w};
-        if (pair < 8)
+        if (pairs[k] < 8)
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            const int r = e * quads + q;
             uint4 o;
             i8x4_to_f16(a[e], o.x, o.y);
             i8x4_to_f16(c[e], o.z, o.w);
-            *reinterpret_cast<uint4 *>(dst + r * 128 + ((pair ^ (r & 7)) << 4)) = o;
+            *reinterpret_cast<uint4 *>(dst + to[k] + e * quads * 128) = o;
           }
       }
       if (h + 1 < halves) load(h + 1);
@@ -411,11 +457,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       s_see[row][w] = v;
     }
-    asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory");
+    // the four warps that share the quadrant's rows
+    auto meet = [&] { asm volatile("bar.sync %0, 128;" ::"r"(1 + (warp & 3)) : "memory"); };
+    meet();
     // position of slot x: x + (x <= turn ? lo_off : hi_off)
     const int turn = ring ? (end - 1) % ring : INT_MAX;
     const int lo_off = ring ? end - 1 - turn : 0, hi_off = lo_off - ring;
-    const bool small = hd <= 256;
     float m = -INFINITY, l = 0.0f;
 
     auto tile = [&](int j, auto is_masked) {
@@ -440,19 +487,28 @@ __global__ void __launch_bounds__(kThreads, 1)
       float top = -INFINITY;
 #pragma unroll
       for (int c = 0; c < kQuarter; c += 4) {
-        const float4 k4 = *reinterpret_cast<const float4 *>(ksq + c);
-        float u[4] = {dot_f32(s[c], small) * k4.x, dot_f32(s[c + 1], small) * k4.y,
-                      dot_f32(s[c + 2], small) * k4.z, dot_f32(s[c + 3], small) * k4.w};
-        if (masked)
+        const ulonglong2 k4 = *reinterpret_cast<const ulonglong2 *>(ksq + c);
+        const uint64_t kk[2] = {k4.x, k4.y};
 #pragma unroll
-          for (int k = 0; k < 4; k++)
-            if (!((seen >> (c + k)) & 1)) u[k] = -INFINITY;
-        top = fmaxf(fmaxf(top, fmaxf(u[0], u[1])), fmaxf(u[2], u[3]));
-#pragma unroll
-        for (int k = 0; k < 4; k++) s[c + k] = __float_as_uint(u[k]);
+        for (int k = 0; k < 4; k += 2) {
+          // int32 to f32: small ones through the mantissa of 1.5 * 2^23, which
+          // spares the unit that also takes the exponentials
+          const uint64_t d =
+              SMALL ? add2(pair2(__uint_as_float(s[c + k] + 0x4B400000u),
+                                 __uint_as_float(s[c + k + 1] + 0x4B400000u)),
+                           pair2(-12582912.0f, -12582912.0f))
+                    : pair2((float)(int)s[c + k], (float)(int)s[c + k + 1]);
+          float u0, u1;
+          split2(mul2(d, kk[k >> 1]), u0, u1);
+          if (masked && !((seen >> (c + k)) & 1)) u0 = -INFINITY;
+          if (masked && !((seen >> (c + k + 1)) & 1)) u1 = -INFINITY;
+          top = fmaxf(top, fmaxf(u0, u1));
+          s[c + k] = __float_as_uint(u0);
+          s[c + k + 1] = __float_as_uint(u1);
+        }
       }
       s_max[buf][quarter][row] = top;
-      asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory");
+      meet();
       top = fmaxf(fmaxf(s_max[buf][0][row], s_max[buf][1][row]),
                   fmaxf(s_max[buf][2][row], s_max[buf][3][row])) * qs;
       // a growing maximum: the sum and, once something was added, the output
@@ -476,35 +532,41 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_wait_st();
       }
       const float ref = m == -INFINITY ? 0.0f : m;
-      float la = 0.0f, lb = 0.0f;
+      const uint64_t qs2 = pair2(qs, qs), ref2 = pair2(-ref, -ref), minus = pair2(-1.0f, -1.0f);
+      uint64_t sum = 0;
 #pragma unroll
       for (int c0 = 0; c0 < kQuarter; c0 += 16) {
         uint32_t hi[8], lo[8];
 #pragma unroll
         for (int c = 0; c < 16; c += 4) {
-          const float4 v4 = *reinterpret_cast<const float4 *>(vsq + c0 + c);
-          const float vv[4] = {v4.x, v4.y, v4.z, v4.w};
-          float w[4];
-#pragma unroll
-          for (int k = 0; k < 4; k++) {
-            const float e = ex2(__fmaf_rn(__uint_as_float(s[c0 + c + k]), qs, -ref));
-            if (k & 1) lb += e;
-            else la += e;
-            w[k] = e * vv[k];
-            // an unseen slot's scale may be anything
-            if (masked && !((seen >> (c0 + c + k)) & 1)) w[k] = 0.0f;
-          }
+          const ulonglong2 v4 = *reinterpret_cast<const ulonglong2 *>(vsq + c0 + c);
+          const uint64_t vv[2] = {v4.x, v4.y};
 #pragma unroll
           for (int k = 0; k < 4; k += 2) {
-            const __half2 h2 = __floats2half2_rn(w[k], w[k + 1]);
+            const int i = c0 + c + k;
+            float e0, e1, w0, w1;
+            split2(fma2(pair2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), qs2, ref2), e0, e1);
+            const uint64_t e = pair2(ex2(e0), ex2(e1));
+            sum = add2(sum, e);
+            uint64_t w = mul2(e, vv[k >> 1]);
+            split2(w, w0, w1);
+            if (masked) {  // an unseen slot's scale may be anything
+              if (!((seen >> i) & 1)) w0 = 0.0f;
+              if (!((seen >> (i + 1)) & 1)) w1 = 0.0f;
+              w = pair2(w0, w1);
+            }
+            const __half2 h2 = __floats2half2_rn(w0, w1);
             const float2 hf = __half22float2(h2);
             hi[(c + k) / 2] = *reinterpret_cast<const uint32_t *>(&h2);
-            lo[(c + k) / 2] = pack2(w[k] - hf.x, w[k + 1] - hf.y);
+            split2(fma2(pair2(hf.x, hf.y), minus, w), w0, w1);
+            lo[(c + k) / 2] = pack2(w0, w1);
           }
         }
         tmem_st_x8(sc + quarter * 16 + c0 / 2, hi);
         tmem_st_x8(sc + 64 + quarter * 16 + c0 / 2, lo);
       }
+      float la, lb;
+      split2(sum, la, lb);
       l += la + lb;
       tmem_wait_st();
     };
@@ -512,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       wait(&bar.sc_full[j & 1], (j >> 1) & 1);
       wait(&bar.s_full[j & 1], (j >> 1) & 1);
       tc::fence_after_sync();
-      if (idle) asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory");
+      if (idle) meet();
       else if (ring || x0 + (j + 1) * kTN > len || x0 + j * kTN < high)
         tile(j, std::true_type());
       else
@@ -523,7 +585,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---- results: the quarters' sums joined, each quarter's dimensions to
     // shared memory, whole rows from there (what the loads filled is free now)
     s_l[quarter][row] = l;
-    asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory");
+    meet();
     const float L = (s_l[0][row] + s_l[1][row]) + (s_l[2][row] + s_l[3][row]);
     wait(&bar.pv_done, (tiles - 1) & 1);
     tc::fence_after_sync();
@@ -546,7 +608,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     tc::fence_before_sync();
     stream::fence_proxy_async_smem();
-    asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory");
+    meet();
     if (quarter == 0 && row < rows) {
       const int h = kvh * G + r - node * G;
       const size_t qr = (size_t)b * p.T + node;
@@ -721,8 +783,10 @@ cudaError_t launch_attend_tile(const TreeParams &p, int num_sms, int *err, cudaS
   tp.err = err;
   CUtensorMap kmap;
   if (!encode_cache_map(&kmap, p.kv)) return cudaErrorInvalidValue;
-  static std::atomic<uint64_t> done{0};
-  cudaError_t e = allow_smem(tile_kernel, kMaxSmem, done);
+  static std::atomic<uint64_t> done[2];
+  const bool small = p.kv.head_dim <= 256;
+  cudaError_t e = small ? allow_smem(tile_kernel<true>, kMaxSmem, done[0])
+                        : allow_smem(tile_kernel<false>, kMaxSmem, done[1]);
   if (e != cudaSuccess) return e;
   const int R = p.T * (p.n_heads / p.kv.kv_heads), rows = R < kTM ? R : kTM;
   const long long all = (long long)p.kv.rows * p.kv.kv_heads * R;
@@ -740,7 +804,8 @@ cudaError_t launch_attend_tile(const TreeParams &p, int num_sms, int *err, cudaS
   cfg.gridDim = dim3((unsigned)grid_of(p.kv, q.items, kTN, num_sms));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = q.smem;
-  if ((e = cudaLaunchKernelEx(&cfg, tile_kernel, tp, kmap)) != cudaSuccess) return e;
+  e = cudaLaunchKernelEx(&cfg, small ? tile_kernel<true> : tile_kernel<false>, tp, kmap);
+  if (e != cudaSuccess) return e;
   const int per = kJoin / (q.dv / 4), groups = (rows + per - 1) / per;
   cfg.gridDim = dim3((unsigned)(q.items * groups));
   cfg.blockDim = dim3(kJoin);

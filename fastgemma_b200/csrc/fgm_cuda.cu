@@ -1795,7 +1795,8 @@ int fgm_cuda_attend_accum_q8(const fgm_cuda_kv *kv, const float *q, int q_ld, in
   if (!lse || !kv->acc) return fail(FGM_CUDA_EINVAL, "attend_accum: null pointer (lse, kv->acc)");
   DevInfo *di = nullptr;
   if ((rc = dev_info(&di))) return rc;
-  return glue_done(launch_attend_accum(p, di->sms, (cudaStream_t)stream), "attend_accum launch");
+  return glue_done(launch_attend_accum(p, di->sms, di->err, (cudaStream_t)stream),
+                   "attend_accum launch");
 }
 
 int fgm_cuda_attend_acc_q8(const fgm_cuda_kv *kv, const float *q, int q_ld, int n_heads,

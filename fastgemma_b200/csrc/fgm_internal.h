@@ -191,7 +191,12 @@ cudaError_t launch_attend_tree(const TreeParams &p, int num_sms, int *err, cudaS
 // kvtile.cu, more than 16 query rows per KV head; err: set when a wait gives up
 size_t attend_tile_workspace(const fgm_cuda_kv &kv, int n_heads, int T);
 cudaError_t launch_attend_tile(const TreeParams &p, int num_sms, int *err, cudaStream_t st);
-cudaError_t launch_attend_accum(const TreeParams &p, int num_sms, cudaStream_t st);
+// kvaccum.cu; launch_quant_rows: int8 queries in blocks of 128 rows, with
+// scales for the attention (qs) or scales and -lse for the accumulation (cst)
+size_t accum_workspace(const fgm_cuda_kv &kv, int n_heads, int T);
+cudaError_t launch_attend_accum(const TreeParams &p, int num_sms, int *err, cudaStream_t st);
+cudaError_t launch_quant_rows(const TreeParams &p, int blocks, int nkb, int8_t *q8, float *qs,
+                              float *cst, cudaStream_t st);
 cudaError_t launch_attend_acc(const TreeParams &p, int num_sms, cudaStream_t st);
 cudaError_t launch_tree_mask(uint64_t *mask, int32_t *pos, const int32_t *parent,
                              const int32_t *lens, int rows, int T, cudaStream_t st);

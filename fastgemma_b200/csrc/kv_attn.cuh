@@ -5,6 +5,8 @@
 
 #include <atomic>
 
+#include <cuda_fp16.h>
+
 #include "fgm_internal.h"
 #include "kv_common.cuh"
 
@@ -29,6 +31,18 @@ __device__ __forceinline__ float ex2(float v) {
 // 2^e for -126 <= e <= 127.
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
 
+// Four int8 as two pairs of f16, exact: 1024 + (v + 128) has v in its low
+// mantissa byte, minus 1152.
+__device__ __forceinline__ void i8x4_to_f16(uint32_t w, uint32_t &lo, uint32_t &hi) {
+  w ^= 0x80808080u;
+  const __half2 off = __floats2half2_rn(1152.0f, 1152.0f);
+  uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+  __half2 x = __hsub2(*reinterpret_cast<__half2 *>(&a), off);
+  __half2 y = __hsub2(*reinterpret_cast<__half2 *>(&b), off);
+  lo = *reinterpret_cast<uint32_t *>(&x);
+  hi = *reinterpret_cast<uint32_t *>(&y);
+}
+
 // Whether a row's node sees position t (node: -1 for a padding row).
 __device__ __forceinline__ bool sees(const TreeParams &p, int b, int node, int len, int t,
                                      int low) {
@@ -48,6 +62,8 @@ __device__ __forceinline__ bool sees(const TreeParams &p, int b, int node, int l
 struct Span {
   int len, first, end;
 };
+// ALL: from the first slot on, seen or not.
+template <bool ALL = false>
 __device__ __forceinline__ Span span_of(const TreeParams &p, int b) {
   Span s;
   s.len = committed(p.kv, p.lens, b, p.T);
@@ -55,7 +71,7 @@ __device__ __forceinline__ Span span_of(const TreeParams &p, int b) {
   s.first = 0;
   if (p.kv.ring) {
     s.end = min(s.end, p.kv.ring);
-  } else if (p.window) {
+  } else if (!ALL && p.window) {
     int low = INT_MAX;
     if (p.pos)
       for (int i = 0; i < p.T; i++) low = min(low, lowest(p.pos[b * p.T + i], p.window));
@@ -86,26 +102,27 @@ __device__ __forceinline__ int tiles_of(const Span &s, int tile) {
   return (s.end - s.first + tile - 1) / tile;
 }
 
+template <bool ALL = false>
 __device__ __forceinline__ bool find_work(const TreeParams &p, int tile, int per_b, int min_per,
                                           int lane, Work &w) {
   const int rows = p.kv.rows, grid = gridDim.x, cta = blockIdx.x;
-  const Span mine = span_of(p, min(lane, rows - 1));
+  const Span mine = span_of<ALL>(p, min(lane, rows - 1));
   const int n0 = lane < rows ? tiles_of(mine, tile) : 0;  // the first 32 sequences stay here
   int total = n0;
-  for (int b = lane + 32; b < rows; b += 32) total += tiles_of(span_of(p, b), tile);
+  for (int b = lane + 32; b < rows; b += 32) total += tiles_of(span_of<ALL>(p, b), tile);
   total = __reduce_add_sync(0xffffffffu, total);
   const long long units = (long long)total * per_b;
   int per = max(min_per, (int)((units + grid - 1) / grid));
   for (;; per += 1 + per / 32) {
     int c = (n0 + per - 1) / per;
     for (int b = lane + 32; b < rows; b += 32)
-      c += (tiles_of(span_of(p, b), tile) + per - 1) / per;
+      c += (tiles_of(span_of<ALL>(p, b), tile) + per - 1) / per;
     if (__reduce_add_sync(0xffffffffu, c) * per_b <= grid) break;
   }
   int base = 0;
   for (int b0 = 0; b0 < rows; b0 += 32) {
     const int b = b0 + lane;
-    const Span s = b0 == 0 ? mine : span_of(p, min(b, rows - 1));
+    const Span s = b0 == 0 ? mine : span_of<ALL>(p, min(b, rows - 1));
     const int tiles = b < rows ? tiles_of(s, tile) : 0, cnt = (tiles + per - 1) / per;
     int inc = cnt * per_b;
 #pragma unroll

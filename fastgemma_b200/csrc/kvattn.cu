@@ -4,6 +4,8 @@
 // R = T * G query rows share one KV head's K and V (T nodes, G query heads
 // per KV head).  Per row: s = (q8 . k8) * qs * ks over the visible slots,
 // p = exp(s - max), out = sum p vs v8 / sum p.
+#include <algorithm>
+
 #include <cuda_fp16.h>
 
 #include "fgm_common.cuh"
@@ -54,18 +56,6 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-// Four int8 as two pairs of f16, exact: 1024 + (v + 128) has v in its low
-// mantissa byte, minus 1152.
-__device__ __forceinline__ void i8x4_to_f16(uint32_t w, uint32_t &lo, uint32_t &hi) {
-  w ^= 0x80808080u;
-  const __half2 off = __floats2half2_rn(1152.0f, 1152.0f);
-  uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
-  __half2 x = __hsub2(*reinterpret_cast<__half2 *>(&a), off);
-  __half2 y = __hsub2(*reinterpret_cast<__half2 *>(&b), off);
-  lo = *reinterpret_cast<uint32_t *>(&x);
-  hi = *reinterpret_cast<uint32_t *>(&y);
 }
 
 // ------------------------------------------------------- few rows: streaming
@@ -471,56 +461,6 @@ __global__ void __launch_bounds__(kAdd) add_weights_kernel(const __grid_constant
     if (x + k <= len) acc[k] = old[k] + sum[k];
 }
 
-// --------------------------------------------------------------- accumulation
-constexpr int kMaxHd = 512;
-
-// Warp: int8 copy of one query head in shared memory, its scale returned.
-__device__ float quant_head(const float *q, int hd, int8_t *q8, int lane) {
-  float top = 0.0f;
-  for (int d = lane; d < hd; d += 32) top = fmaxf(top, q_abs(q[d]));
-  top = warp_max(top);
-  const float inv = q_inv(top);
-  for (int d = lane; d < hd; d += 32) q8[d] = (int8_t)q_int8(q[d], inv);
-  __syncwarp();
-  return q_scale(top);
-}
-
-// One warp per slot: all nodes and heads in order.
-__global__ void __launch_bounds__(128) accum_kernel(const TreeParams p) {
-  __shared__ __align__(16) int8_t q8[4][kMaxHd];
-  const int hd = p.kv.head_dim, kvd = p.kv.kv_heads * hd, b = blockIdx.y;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int x = blockIdx.x * 4 + warp;
-  const int len = committed(p.kv, p.lens, b, p.T), end = len + p.T;
-  const int t = pos_of(p.kv.ring, x, end);
-  if (x >= p.kv.cap || t < 0) return;
-  const int G = p.n_heads / p.kv.kv_heads;
-  const float ks = p.kv.ks[(size_t)b * p.kv.ks_stride + x];
-  float sum = 0.0f;
-  for (int i = 0; i < p.T; i++) {
-    const int r = b * p.T + i;
-    if (p.take && !p.take[r]) continue;
-    if (!sees(p, b, i, len, t, lowest(p.pos ? p.pos[r] : len + i, p.window))) continue;
-    for (int h = 0; h < p.n_heads; h++) {
-      const float lse = p.lse[r * p.lse_row + h * p.lse_head];
-      if (lse == -INFINITY) continue;
-      const float qs = quant_head(p.q + (size_t)r * p.q_ld + (size_t)h * hd, hd, q8[warp], lane);
-      const int8_t *kr = p.kv.kc + (size_t)b * p.kv.kc_stride + (size_t)x * kvd + (h / G) * hd;
-      int dot = 0;
-      for (int d = lane * 4; d < hd; d += 128)
-        dot = __dp4a(*reinterpret_cast<const int *>(kr + d),
-                     *reinterpret_cast<const int *>(&q8[warp][d]), dot);
-      dot = __reduce_add_sync(0xffffffffu, dot);
-      __syncwarp();
-      sum += expf(__fmul_rn(__fmul_rn((float)dot, qs), ks) - lse);
-    }
-  }
-  if (lane == 0) {
-    float *a = p.kv.acc + (size_t)b * p.kv.acc_stride + x;
-    *a = (t < len ? p.decay * *a : 0.0f) + sum;
-  }
-}
-
 // ------------------------------------------------------------------ launching
 // Row blocks of 8 * nt rows: one block of 16 where the accumulators of 16
 // rows fit the registers (head_dim <= 256), else blocks of 8.
@@ -616,19 +556,14 @@ cudaError_t launch_stream(const TreeParams &p, bool accumulate, int num_sms, cud
 bool streams(const fgm_cuda_kv &kv, int n_heads, int T) { return T * (n_heads / kv.kv_heads) <= 16; }
 
 size_t attend_workspace(const fgm_cuda_kv &kv, int n_heads, int T) {
-  return streams(kv, n_heads, T) ? ws_of(kv, n_heads, T).total
-                                 : attend_tile_workspace(kv, n_heads, T);
+  const size_t n = streams(kv, n_heads, T) ? ws_of(kv, n_heads, T).total
+                                           : attend_tile_workspace(kv, n_heads, T);
+  return std::max(n, accum_workspace(kv, n_heads, T));
 }
 
 cudaError_t launch_attend_tree(const TreeParams &p, int num_sms, int *err, cudaStream_t st) {
   if (!streams(p.kv, p.n_heads, p.T)) return launch_attend_tile(p, num_sms, err, st);
   return launch_stream(p, false, num_sms, st);
-}
-
-cudaError_t launch_attend_accum(const TreeParams &p, int num_sms, cudaStream_t st) {
-  const int slots = p.kv.ring ? p.kv.ring : p.kv.cap;
-  accum_kernel<<<dim3((unsigned)((slots + 3) / 4), (unsigned)p.kv.rows), 128, 0, st>>>(p);
-  return cudaGetLastError();
 }
 
 cudaError_t launch_attend_acc(const TreeParams &p, int num_sms, cudaStream_t st) {

@@ -23,26 +23,18 @@
 // instead of being staged as int8.
 #include <type_traits>
 
-#include <cuda_fp16.h>
-
-#include "fgm_internal.h"
-#include "kv_attn.cuh"
-#include "stream_ptx.cuh"
-#include "tc_ptx.cuh"
+#include "kv_tc.cuh"
 
 namespace fgm {
 namespace {
 
 using namespace kv;
 
-constexpr int kTM = 128;          // query rows per tile
-constexpr int kTN = 128;          // slots per tile
 constexpr int kHalf = 64;         // slots per V stage
 constexpr int kVStages = 3;
 constexpr int kSoftWarps = 16, kSoft = kSoftWarps * 32;
 constexpr int kThreads = 128 + kSoft + 128;  // loads and MMAs, softmax, V conversion
 constexpr int kQuarter = kTN / 4;  // slots of a softmax thread
-constexpr int kChunk = 128 * 128; // bytes of one 128-byte column of Q or of a K tile
 constexpr int kGrow = 8;          // log2 by which a row's maximum may grow unnoticed
 constexpr int kUnit = 5;          // f16 weights: p * vs * 2^(kUnit - ve), at most 2^(kUnit + kGrow)
 constexpr uint32_t kColS = 256;   // TMEM columns: output [0, 256), scores / weights 2 x 128
@@ -59,134 +51,6 @@ struct TileParams {
   int2 *desc;              // [items]: first CTA, CTAs
   int *err;
 };
-
-__device__ __forceinline__ uint64_t desc128(uint32_t a) { return tc::sdesc_sw128(a); }
-
-// D[tmem] (+)= A[tmem, f16] * B[smem desc, f16], f32 accumulate.
-__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
-                                           uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
-// D f32, A and B f16, both K-major.
-__host__ __device__ constexpr uint32_t idesc_f16(int m, int n) {
-  return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
-}
-
-__device__ __forceinline__ void tmem_st_x8(uint32_t a, const uint32_t (&r)[8]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(a), "r"(r[0]),
-      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-      : "memory");
-}
-
-__device__ __forceinline__ void tmem_ld_x8(uint32_t a, uint32_t (&r)[8]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-                 "=r"(r[7])
-               : "r"(a));
-}
-
-__device__ __forceinline__ void tmem_ld_x2(uint32_t a, uint32_t (&r)[2]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0,%1}, [%2];"
-               : "=r"(r[0]), "=r"(r[1])
-               : "r"(a));
-}
-
-// One row of results to global memory (bulk group of the thread).
-__device__ __forceinline__ void bulk_s2g(void *dst, const void *src, uint32_t bytes) {
-  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst),
-               "r"(tc::smem_u32(src)), "r"(bytes)
-               : "memory");
-}
-
-__device__ __forceinline__ void tmem_wait_st() {
-  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-}
-
-// Bits [a, b) of a 64-bit word, whatever a and b.
-__device__ __forceinline__ uint64_t bit_range(int a, int b) {
-  a = max(a, 0);
-  b = min(b, 64);
-  return a >= b ? 0 : (~0ull >> (64 - (b - a))) << a;
-}
-
-// Which of the positions t .. t + 31 a row sees: committed ones from `low` on,
-// nodes by its words.
-__device__ __forceinline__ uint32_t seen_from(int t, int len, int low, const uint64_t (&nodes)[4]) {
-  uint32_t v = (uint32_t)bit_range(max(low, 0) - t, len - t);
-  const int n = t - len;  // node of bit 0
-  if (n > -32 && n < FGM_CUDA_TREE_MAX) {
-    if (n < 0) {
-      v |= (uint32_t)(nodes[0] << -n);
-    } else {
-      const int w = n >> 6, s = n & 63;
-      v |= (uint32_t)(nodes[w] >> s);
-      if (w < 3 && s > 32) v |= (uint32_t)(nodes[w + 1] << (64 - s));
-    }
-  }
-  return v;
-}
-
-// Two f32 in one register pair: the packed forms of the FP32 pipe.
-__device__ __forceinline__ uint64_t pair2(float a, float b) {
-  uint64_t d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
-  return d;
-}
-__device__ __forceinline__ void split2(uint64_t d, float &a, float &b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(d));
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t *>(&h);
-}
-
-// Four int8 as two f16 pairs, exact (see the streaming kernel).
-__device__ __forceinline__ void i8x4_to_f16(uint32_t w, uint32_t &lo, uint32_t &hi) {
-  w ^= 0x80808080u;
-  const __half2 off = __floats2half2_rn(1152.0f, 1152.0f);
-  uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
-  const __half2 x = __hsub2(*reinterpret_cast<__half2 *>(&a), off);
-  const __half2 y = __hsub2(*reinterpret_cast<__half2 *>(&b), off);
-  lo = *reinterpret_cast<const uint32_t *>(&x);
-  hi = *reinterpret_cast<const uint32_t *>(&y);
-}
-
-// mbarrier test that may put the warp to sleep for up to 10 us: what waits for
-// long should not take issue slots from what works.
-__device__ __forceinline__ bool mbar_sleep(uint64_t *bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(tc::smem_u32(bar)), "r"(parity), "r"(10000u)
-      : "memory");
-  return ok != 0;
-}
 
 struct Bars {
   uint64_t q_full, k_full[4], k_empty[4], v_full[kVStages], v_empty[kVStages], s_full[2], p_full[2],
@@ -635,45 +499,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// A warp per query row: its int8 copy in the block's swizzled place, its scale
-// times log2(e).
-constexpr int kQuantRows = 8;
-__global__ void __launch_bounds__(kQuantRows * 32)
-    quant_rows_kernel(const __grid_constant__ TreeParams p, int blocks, int nkb, int8_t *q8,
-                      float *qs) {
-  const int lane = threadIdx.x & 31, row = blockIdx.x * kQuantRows + (threadIdx.x >> 5);
-  const int hd = p.kv.head_dim, G = p.n_heads / p.kv.kv_heads, R = p.T * G;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int bk = row / R, r = row - bk * R, b = bk / p.kv.kv_heads, kvh = bk - b * p.kv.kv_heads;
-  if (b >= p.kv.rows) return;
-  const int node = r / G;
-  const float4 *src = reinterpret_cast<const float4 *>(
-      p.q + ((size_t)b * p.T + node) * p.q_ld + (size_t)(kvh * G + r - node * G) * hd);
-  float4 v[4];
-  float top = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    v[i] = lane + 32 * i < hd / 4 ? src[lane + 32 * i] : make_float4(0, 0, 0, 0);
-    top = fmaxf(fmaxf(top, fmaxf(q_abs(v[i].x), q_abs(v[i].y))),
-                fmaxf(q_abs(v[i].z), q_abs(v[i].w)));
-  }
-  top = warp_max(top);
-  const float inv = q_inv(top);
-  const size_t block = (size_t)bk * blocks + r / kTM;
-  const int j = r % kTM;
-  int8_t *dst = q8 + block * nkb * kChunk + j * 128 + (((lane >> 2) ^ (j & 7)) << 4) + (lane & 3) * 4;
-#pragma unroll
-  for (int i = 0; i < 4; i++)
-    if (lane + 32 * i < hd / 4)
-      *reinterpret_cast<uint32_t *>(dst + i * kChunk) =
-          (q_int8(v[i].x, inv) & 255) | (q_int8(v[i].y, inv) & 255) << 8 |
-          (q_int8(v[i].z, inv) & 255) << 16 | q_int8(v[i].w, inv) << 24;
-  // never 0, so that a masked score stays -inf (a zero query's dots are 0)
-  if (lane == 0)
-    qs[block * kTM + j] =
-        fmaxf(q_scale(top) * kLog2e, 1e-37f) + (top < INFINITY ? 0.0f : q_scale(top));
-}
-
 // Joins an item's partial results: a CTA takes a few rows, a thread four
 // dimensions of one.  The first parts' values are asked for together with
 // their statistics.
@@ -789,11 +614,9 @@ cudaError_t launch_attend_tile(const TreeParams &p, int num_sms, int *err, cudaS
                         : allow_smem(tile_kernel<false>, kMaxSmem, done[1]);
   if (e != cudaSuccess) return e;
   const int R = p.T * (p.n_heads / p.kv.kv_heads), rows = R < kTM ? R : kTM;
-  const long long all = (long long)p.kv.rows * p.kv.kv_heads * R;
-  quant_rows_kernel<<<(unsigned)((all + kQuantRows - 1) / kQuantRows), kQuantRows * 32, 0, st>>>(
-      p, q.blocks, q.nkb, reinterpret_cast<int8_t *>(ws + q.q8),
-      reinterpret_cast<float *>(ws + q.qs));
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  e = launch_quant_rows(p, q.blocks, q.nkb, reinterpret_cast<int8_t *>(ws + q.q8),
+                        reinterpret_cast<float *>(ws + q.qs), nullptr, st);
+  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -46,6 +46,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ float s_sum[2][4][kTN];
   __shared__ int s_low[FGM_CUDA_TREE_MAX];
   __shared__ uint64_t s_see[FGM_CUDA_TREE_MAX][4];  // nodes that each node sees
+  __shared__ uint64_t s_by[kTN][4];                 // nodes that see each slot of a tile
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort, s_high;
   const TreeParams &p = ap.t;
@@ -207,6 +208,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float *ks = p.kv.ks + (size_t)b * p.kv.ks_stride;
     float *acc = p.kv.acc + (size_t)b * p.kv.acc_stride;
     const int high = s_high;
+    // the four warps that share the quadrant's slots
+    auto meet = [&] { asm volatile("bar.sync %0, 128;" ::"r"(1 + (warp & 3)) : "memory"); };
     int u = 0;
     for (int t = t0; t < t1; t++) {
       const int x = t * kTN + in_tile, pos = x < x1 ? pos_of(ring, x, end) : -1;
@@ -222,8 +225,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float *ca = &s_cst[buf][0][c0], *cz = &s_cst[buf][1][c0];
         const uint64_t k2 = pair2(scale, scale), l2 = pair2(kLog2e, kLog2e);
         uint64_t add = 0;
-        int node = 0, g = 0;
-        if (masked) node = (blk * kTM + c0) / G, g = (blk * kTM + c0) - node * G;
+        // the nodes of these rows as bits from the first row's node on
+        uint64_t by = 0;
+        int g = 0;
+        if (masked) {
+          const int n = (blk * kTM + c0) / G, w = n >> 6, sh = n & 63;
+          g = blk * kTM + c0 - n * G;
+          by = s_by[in_tile][w] >> sh;
+          if (w < 3 && sh) by |= s_by[in_tile][w + 1] << (64 - sh);
+        }
         tc::tmem_wait_ld();
 #pragma unroll
         for (int c = 0; c < kQuarter; c += 4) {
@@ -244,16 +254,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             e0 = ex2(e0);
             e1 = ex2(e1);
             if (masked) {
-              bool v[2];
-#pragma unroll
-              for (int e = 0; e < 2; e++) {
-                const int n = min(node, p.T - 1);
-                v[e] = pos >= 0 && (pos < len ? pos >= s_low[n]
-                                              : (s_see[n][(pos - len) >> 6] >> ((pos - len) & 63)) & 1);
-                if (++g == G) g = 0, node++;
-              }
-              if (!v[0]) e0 = 0.0f;
-              if (!v[1]) e1 = 0.0f;
+              if (!(by & 1)) e0 = 0.0f;
+              if (++g == G) g = 0, by >>= 1;
+              if (!(by & 1)) e1 = 0.0f;
+              if (++g == G) g = 0, by >>= 1;
             }
             add = add2(add, pair2(e0, e1));
           }
@@ -264,6 +268,25 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       if (t >= first) {
         const bool masked = ring || (t + 1) * kTN > len || t * kTN < high;
+        if (masked) {  // which nodes see this slot, 64 of them per quarter
+          uint64_t v = 0;
+          const int w0 = quarter * 64, n = min(64, p.T - w0), j = pos - len;
+          if (pos >= 0 && n > 0) {
+            if (pos < len && !p.window) {
+              v = ~0ull;
+            } else if (pos < len) {
+              for (int i = 0; i < n; i++) v |= (uint64_t)(pos >= s_low[w0 + i]) << i;
+            } else if (!p.mask && !p.window) {
+              v = bit_range(j - w0, n);
+            } else {
+              const uint64_t *see = &s_see[w0][j >> 6];
+#pragma unroll 8
+              for (int i = 0; i < n; i++) v |= ((see[i * 4] >> (j & 63)) & 1) << i;
+            }
+          }
+          s_by[in_tile][quarter] = v;
+          meet();
+        }
         for (int kvh = 0; kvh < kvh_n; kvh++)
           for (int blk = 0; blk < ap.blocks; blk++, u++) {
             const int buf = u % kBufs;
@@ -279,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
       }
       s_sum[t & 1][quarter][in_tile] = sum;
-      asm volatile("bar.sync %0, 128;" ::"r"(1 + (warp & 3)) : "memory");
+      meet();
       if (quarter == 0 && pos >= 0)
         acc[x] = old + ((sum + s_sum[t & 1][1][in_tile]) +
                         (s_sum[t & 1][2][in_tile] + s_sum[t & 1][3][in_tile]));

@@ -1,7 +1,11 @@
 // Trees of drafted tokens and the moves of cache rows: ancestor masks, greedy
 // verification, the commit of an accepted path, eviction to a budget.
+#include <cooperative_groups.h>
+
 #include "fgm_internal.h"
 #include "kv_attn.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace fgm {
 namespace {
@@ -168,7 +172,7 @@ struct EvictParams {
 };
 
 constexpr int kPlanThreads = 1024;
-constexpr int kEvictMax = 524288;
+constexpr int kMaxPlanSmem = 200 * 1024;
 
 // Order of acc as unsigned: not-a-number 0, then ascending, -0 equal to 0.
 __device__ __forceinline__ uint32_t rank_key(float v) {
@@ -177,23 +181,35 @@ __device__ __forceinline__ uint32_t rank_key(float v) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// One CTA per sequence.  The budget-th largest key comes from four passes of
-// 256 counters over its bytes; then every warp walks its own run of slots,
-// 32 at a time, and leaves the kept ones as a bitmask in shared memory with
-// the number kept before each word, from which every slot below the budget
-// finds its source.  Bound by latency: a handful of passes over keys that lie
-// in shared memory (CACHED: up to kCachedKeys slots; longer caches read acc
-// and tpos again in each pass).
-constexpr int kCachedKeys = 40960;
+// A cluster of CTAs per sequence, a run of slots each.  The budget-th largest
+// key comes from four passes of 256 counters over its bytes, summed over the
+// cluster through distributed shared memory; then every warp walks its share
+// of the run, 32 slots at a time, and leaves the kept ones as a bitmask with
+// the number kept before each word.  Kept slots past the budget write
+// themselves, by rank, into a list spread over the cluster (where the keys
+// were); the evicted slots below it read their source there.  Bound by
+// latency: eight cluster barriers and a pass or two over the slots for each,
+// which is why a run is short (kRunSlots) and its keys stay in shared memory
+// (CACHED; longer runs read acc and tpos again in every pass).
+constexpr int kRunSlots = 2048, kCachedKeys = 40960;
 
-template <bool CACHED>
+constexpr int kMaxCluster = 8;
+
+template <bool CACHED, bool CLUSTER>
 __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictParams p) {
-  extern __shared__ uint32_t smem[];  // bits [words], kept before each word [words], keys
-  __shared__ unsigned hist[256];
-  __shared__ int s_warp[kPlanThreads / 32], s_base[kPlanThreads / 32 + 1];
+  extern __shared__ uint32_t smem[];  // bits [words], kept before each word [words], keys / list
+  __shared__ unsigned hist[4][256], total[256];
+  __shared__ int s_warp[kPlanThreads / 32], s_newest, s_eq, s_kept, s_kept_low;
   __shared__ uint32_t s_prefix;
-  __shared__ int s_left, s_newest;
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  __shared__ int s_left;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = CLUSTER ? (int)cluster.num_blocks() : 1;
+  const int rank = CLUSTER ? (int)cluster.block_rank() : 0;
+  auto sync = [&] {
+    if (CLUSTER) cluster.sync();
+    else __syncthreads();
+  };
+  const int b = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int n = committed(p.kv, p.lens, b, 0), budget = p.budget;
   const float *acc = p.kv.acc + (size_t)b * p.kv.acc_stride;
@@ -201,66 +217,85 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictPar
   int32_t *map = p.map + (size_t)b * budget;
   float *ao = p.acc_out + (size_t)b * p.acc_stride;
   int32_t *to = p.tpos_out ? p.tpos_out + (size_t)b * p.tpos_stride : nullptr;
-  if (tid == 0) p.lens_out[b] = min(n, budget);
   // a slot's own words to where they go; in place the sources lie past the budget
   auto place = [&](int x, int s) {
     if (s != x || ao != acc) ao[x] = acc[s];
     if (to && (s != x || to != tp)) to[x] = tp ? tp[s] : s;
   };
   if (n <= budget) {
-    for (int x = tid; x < budget; x += kPlanThreads) {
+    for (int x = rank * kPlanThreads + tid; x < budget; x += C * kPlanThreads) {
       map[x] = x < n ? x : -1;
       if (x < n) place(x, x);
     }
+    if (rank == 0 && tid == 0) p.lens_out[b] = n;
     return;
   }
-  const int words = (n + 31) / 32, per_warp = (words + kPlanThreads / 32 - 1) / (kPlanThreads / 32);
+  const int words = ((n + C - 1) / C + 31) / 32, run = words * 32;  // of one CTA
+  // list entries of one CTA: at most half of the slots are kept past the budget
+  // (each fills an evicted one below it)
+  const int part = run / 2;
+  const int first = min(n, rank * run), last = min(n, first + run);
+  const int per_warp = (words + kPlanThreads / 32 - 1) / (kPlanThreads / 32);
   uint32_t *bits = smem, *before = smem + words, *keys = before + words;
+  // a word of every CTA of the cluster, all asked for at once (0 past the last)
+  auto all = [&](int *w, int (&v)[kMaxCluster]) {
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; r++)
+      v[r] = !CLUSTER ? (r == 0 ? *w : 0) : r < C ? *cluster.map_shared_rank(w, r) : 0;
+  };
+  auto entry = [&](int i) {  // of the list
+    return CLUSTER ? cluster.map_shared_rank(keys, i / part) + i % part : keys + i;
+  };
 
   // the newest position (the slot's index where no positions are kept)
-  if (tid == 0) s_newest = tp ? INT_MIN : n - 1;
-  if (tid < 256) hist[tid] = 0;
+  if (tid == 0) s_newest = INT_MIN;
+  for (int i = tid; i < 4 * 256; i += kPlanThreads) (&hist[0][0])[i] = 0;
   __syncthreads();
+  int newest = n - 1;
   if (tp) {
-    int newest = INT_MIN;
-#pragma unroll 8
-    for (int x = tid; x < n; x += kPlanThreads) newest = max(newest, tp[x]);
+    newest = INT_MIN;
+#pragma unroll 4
+    for (int x = first + tid; x < last; x += kPlanThreads) newest = max(newest, tp[x]);
     newest = __reduce_max_sync(0xffffffffu, newest);
     if (lane == 0) atomicMax(&s_newest, newest);
-    __syncthreads();
+    sync();
+    int v[kMaxCluster];
+    all(&s_newest, v);
+    newest = v[0];
+#pragma unroll
+    for (int r = 1; r < kMaxCluster; r++)
+      if (r < C) newest = max(newest, v[r]);
   }
-  const long long old = (long long)s_newest - p.recent;
+  const long long old = (long long)newest - p.recent;
   auto make_key = [&](int x) -> uint32_t {
     const int t = tp ? tp[x] : x;
     return t < p.sink || t > old ? 0xFFFFFFFFu : rank_key(acc[x]);
   };
-  if (CACHED) {
-#pragma unroll 4
-    for (int x = tid; x < n; x += kPlanThreads) {
-      const uint32_t k = make_key(x);
-      keys[x] = k;
-      atomicAdd(&hist[k >> 24], 1u);
-    }
-  }
-  auto key = [&](int x) -> uint32_t { return CACHED ? keys[x] : make_key(x); };
+  auto key = [&](int x) -> uint32_t { return CACHED ? keys[x - first] : make_key(x); };
 
   uint32_t prefix = 0;
   int left = budget;  // keys still to take among those that share the prefix
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (!CACHED || shift < 24) {
+  for (int pass = 0; pass < 4; pass++) {
+    const int shift = 24 - 8 * pass;
 #pragma unroll 4
-      for (int x = tid; x < n; x += kPlanThreads) {
-        const uint32_t k = key(x);
-        if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8)))
-          atomicAdd(&hist[(k >> shift) & 255], 1u);
-      }
+    for (int x = first + tid; x < last; x += kPlanThreads) {
+      const uint32_t k = pass == 0 ? make_key(x) : key(x);
+      if (CACHED && pass == 0) keys[x - first] = k;
+      if (pass == 0 || (k >> (shift + 8)) == (prefix >> (shift + 8)))
+        atomicAdd(&hist[pass][(k >> shift) & 255], 1u);
+    }
+    sync();
+    if (tid < 256) {
+      int v[kMaxCluster];
+      all(reinterpret_cast<int *>(&hist[pass][tid]), v);
+      total[tid] = (unsigned)(((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7])));
     }
     __syncthreads();
     if (warp == 0) {  // the digit, from the largest down: 8 counters a lane
       int c[8], sum = 0;
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        c[i] = (int)hist[255 - 8 * lane - i];
+        c[i] = (int)total[255 - 8 * lane - i];
         sum += c[i];
       }
       int inc = sum;
@@ -286,81 +321,99 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictPar
     __syncthreads();
     prefix = s_prefix;
     left = s_left;
-    if (tid < 256) hist[tid] = 0;
-    __syncthreads();
   }
 
   // keys above the threshold stay, and of the equal ones the first `left`
   const int w0 = min(words, warp * per_warp), w1 = min(words, w0 + per_warp);
+  // of the warps' numbers: their sum and, in s_warp, what lies before each warp
+  auto scan_warps = [&](int count) {
+    if (lane == 0) s_warp[warp] = count;
+    __syncthreads();
+    int sum = 0;
+    if (warp == 0) {
+      const int c = s_warp[lane];
+      int inc = c;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+      }
+      s_warp[lane] = inc - c;
+      sum = __shfl_sync(0xffffffffu, inc, 31);
+    }
+    return sum;  // of thread 0
+  };
   int count = 0;
-#pragma unroll 4
   for (int w = w0; w < w1; w++) {
-    const int x = w * 32 + lane;
-    count += __popc(__ballot_sync(0xffffffffu, x < n && key(x) == prefix));
+    const int x = first + w * 32 + lane;
+    count += __popc(__ballot_sync(0xffffffffu, x < last && key(x) == prefix));
   }
-  if (lane == 0) s_warp[warp] = count;
+  int sum = scan_warps(count);
+  if (tid == 0) s_eq = sum;
+  sync();
+  int seen = s_warp[warp];  // equal keys before this warp's
+  int v[kMaxCluster], lows[kMaxCluster];
+  all(&s_eq, v);
+#pragma unroll
+  for (int r = 0; r < kMaxCluster; r++)
+    if (r < rank) seen += v[r];
   __syncthreads();
-  int rank = 0;
-  for (int w = lane; w < warp; w += 32) rank += s_warp[w];
-  rank = __reduce_add_sync(0xffffffffu, rank);
   count = 0;
-#pragma unroll 4
+  int count_low = 0;
   for (int w = w0; w < w1; w++) {
-    const int x = w * 32 + lane;
-    const uint32_t k = x < n ? key(x) : 0;
-    const unsigned eq = __ballot_sync(0xffffffffu, x < n && k == prefix);
+    const int x = first + w * 32 + lane;
+    const uint32_t k = x < last ? key(x) : 0;
+    const unsigned eq = __ballot_sync(0xffffffffu, x < last && k == prefix);
     const bool keep =
-        x < n && (k > prefix || (k == prefix && rank + __popc(eq & ((1u << lane) - 1)) < left));
+        x < last && (k > prefix || (k == prefix && seen + __popc(eq & ((1u << lane) - 1)) < left));
     const unsigned kept = __ballot_sync(0xffffffffu, keep);
-    rank += __popc(eq);
+    count_low += __popc(__ballot_sync(0xffffffffu, keep && x < budget));
+    seen += __popc(eq);
     if (lane == 0) {
       bits[w] = kept;
       before[w] = count;
     }
     count += __popc(kept);
   }
-  __syncthreads();
-  if (lane == 0) s_warp[warp] = count;
-  __syncthreads();
-  if (warp == 0) {
-    const int c = s_warp[lane];
-    int inc = c;
+  if (tid == 0) s_kept_low = 0;
+  sum = scan_warps(count);  // its barrier comes before the sums below
+  if (tid == 0) s_kept = sum;
+  if (lane == 0 && count_low) atomicAdd(&s_kept_low, count_low);
+  sync();
+  int base = s_warp[warp], low = 0;  // kept before this warp's slots; kept below the budget
+  all(&s_kept, v);
+  all(&s_kept_low, lows);
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += v;
+  for (int r = 0; r < kMaxCluster; r++) {
+    if (r < rank) base += v[r];
+    low += lows[r];
+  }
+  // kept slots past the budget into the list, which takes the keys' place
+  for (int w = w0; w < w1; w++) {
+    const int x = first + w * 32 + lane;
+    const uint32_t word = bits[w];
+    const int at = base + (int)before[w] + __popc(word & ((1u << lane) - 1));
+    __syncwarp();
+    if (lane == 0) before[w] = base + (int)before[w];
+    if (x >= budget && ((word >> lane) & 1)) {
+      const int i = at - low;
+      *entry(i) = (uint32_t)x;
     }
-    s_base[lane + 1] = inc;
-    if (lane == 0) s_base[0] = 0;
   }
-  __syncthreads();
-  {
-    const int base = s_base[warp];
-    for (int w = w0 + lane; w < w1; w += 32) before[w] += base;
-  }
-  __syncthreads();
-  auto kept_before = [&](int x) -> int {
-    return (int)before[x >> 5] + __popc(bits[x >> 5] & ((1u << (x & 31)) - 1));
-  };
-  const int low = kept_before(budget);  // kept slots below the budget (budget < n)
-#pragma unroll 2
-  for (int x = tid; x < budget; x += kPlanThreads) {
+  sync();
+  for (int x = first + tid; x < min(last, budget); x += kPlanThreads) {
+    const int w = (x - first) >> 5;
+    const uint32_t word = bits[w], bit = 1u << (x & 31);
     int s = x;
-    if (!((bits[x >> 5] >> (x & 31)) & 1)) {
-      const int want = low + (x - kept_before(x));  // kept slots before the one that moves here
-      int lo = budget >> 5, hi = words;             // last word with before <= want
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if ((int)before[mid] <= want) lo = mid;
-        else hi = mid;
-      }
-      uint32_t w = bits[lo];
-      for (int k = want - (int)before[lo]; k > 0; k--) w &= w - 1;
-      s = lo * 32 + __ffs(w) - 1;
+    if (!(word & bit)) {  // as many evicted slots lie before it as kept ones before its source
+      const int i = x - ((int)before[w] + __popc(word & (bit - 1)));
+      s = (int)*entry(i);
     }
     map[x] = s;
     place(x, s);
   }
+  sync();  // no CTA leaves while another may read its part of the list
+  if (rank == 0 && tid == 0) p.lens_out[b] = budget;
 }
 
 // A warp per kMoveSlots slots of a sequence: the rows that move, their loads
@@ -448,24 +501,36 @@ cudaError_t launch_kv_evict(const fgm_cuda_kv &kv, const int32_t *lens, int budg
                 out_stride};
   if (!acc_out) p.acc_out = kv.acc, p.acc_stride = kv.acc_stride;
   if (!tpos_out) p.tpos_out = kv.tpos, p.tpos_stride = kv.tpos_stride;
-  // the bitmask, its counts and, where they fit, the keys of a whole cache
-  const bool cached = kv.cap <= kCachedKeys;
-  const size_t words = (size_t)(kv.cap + 31) / 32, smem = words * 8 + (cached ? words * 128 : 0);
-  auto plan = cached ? evict_plan_kernel<true> : evict_plan_kernel<false>;
-  static std::atomic<uint64_t> done[2];
-  cudaError_t e = allow_smem(plan, cached ? kCachedKeys / 32 * 136 : kEvictMax / 32 * 8, done[cached]);
+  // CTAs of a sequence: runs of about kRunSlots, at most a cluster of 8
+  int c = 1;
+  while (c < kMaxCluster && kv.cap > c * kRunSlots) c <<= 1;
+  const int words = ((kv.cap + c - 1) / c + 31) / 32;
+  // the keys' room also takes the list of kept slots past the budget, which
+  // has no more entries than there are evicted ones
+  const bool cached = words * 32 <= kCachedKeys;
+  auto plan = c == 1 ? evict_plan_kernel<true, false>
+              : cached ? evict_plan_kernel<true, true> : evict_plan_kernel<false, true>;
+  static std::atomic<uint64_t> done[3];
+  cudaError_t e = allow_smem(plan, kMaxPlanSmem, done[c == 1 ? 0 : cached ? 1 : 2]);
   if (e != cudaSuccess) return e;
-  plan<<<kv.rows, kPlanThreads, smem, st>>>(p);
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  const int groups = (budget + kMoveSlots - 1) / kMoveSlots;
-  const long long items = (long long)kv.rows * groups;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)c;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = c > 1;
+  cfg.stream = st;
+  cfg.gridDim = dim3((unsigned)(kv.rows * c));
+  cfg.blockDim = dim3(kPlanThreads);
+  cfg.dynamicSmemBytes = (size_t)words * 8 + (size_t)(cached ? words : (words + 1) / 2) * 128;
+  if ((e = cudaLaunchKernelEx(&cfg, plan, p)) != cudaSuccess) return e;
+  const int groups = (budget + kMoveSlots - 1) / kMoveSlots;
+  const long long items = (long long)kv.rows * groups;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cfg.stream = st;
+  cfg.dynamicSmemBytes = 0;
   cfg.gridDim = dim3((unsigned)((items + kMoveWarps - 1) / kMoveWarps));
   cfg.blockDim = dim3(kMoveWarps * 32);
   return cudaLaunchKernelEx(&cfg, evict_move_kernel, p, groups);

@@ -549,7 +549,9 @@ def evict_plan(acc, tpos, n, budget, sink, recent):
     ([1000, 1000], 32, 8, 40, "random"), ([777], 500, 4, 600, "random"),
     ([2049, 1500], 1024, 4, 100, "ties"), ([3000], 2999, 0, 7, "equal"),
     ([1025], 1, 0, 0, "nan"), ([4000, 3999], 2000, 4, 32, "nan"),
-    ([900], 450, 5, 50, "moved"), ([20000], 15000, 4, 1000, "ties")])
+    ([900], 450, 5, 50, "moved"), ([20000], 15000, 4, 1000, "ties"),
+    ([9000, 8193, 40], 8192, 0, 1, "moved"), ([5000, 4999], 2500, 0, 0, "equal"),
+    ([400000], 200000, 4, 1000, "ties")])
 @pytest.mark.parametrize("in_place", [False, True])
 def test_eviction_to_a_budget(lens, budget, sink, recent, kind, in_place):
     rng = np.random.default_rng(sum(lens) + budget + recent)

@@ -33,6 +33,15 @@ __host__ __device__ constexpr uint32_t idesc_f16(int m, int n) {
   return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
+__device__ __forceinline__ void tmem_st_x16(uint32_t a, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(a),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
 __device__ __forceinline__ void tmem_st_x8(uint32_t a, const uint32_t (&r)[8]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(a), "r"(r[0]),
@@ -51,6 +60,13 @@ __device__ __forceinline__ void tmem_ld_x2(uint32_t a, uint32_t (&r)[2]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0,%1}, [%2];"
                : "=r"(r[0]), "=r"(r[1])
                : "r"(a));
+}
+
+template <int N>
+__device__ __forceinline__ void tmem_ld(uint32_t a, uint32_t (&r)[N]) {
+  static_assert(N == 2 || N == 8, "widths in use");
+  if constexpr (N == 8) tmem_ld_x8(a, r);
+  else tmem_ld_x2(a, r);
 }
 
 // One row of results to global memory (bulk group of the thread).
@@ -118,18 +134,27 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// mbarrier test that may put the warp to sleep for up to 10 us: what waits for
-// long should not take issue slots from what works.
-__device__ __forceinline__ bool mbar_sleep(uint64_t *bar, uint32_t parity) {
+// Waits until the phase with `parity` is over.  The tests put the warp to sleep
+// for up to 10 us each: spinning, or reading a clock or the abort word between
+// the tests, takes issue slots from the warps that work (chunk_256_16k 61.7 us
+// like this, 65 to 71 otherwise).  After kWaitTests tests, two seconds asleep,
+// the wait gives up and raises the abort word, on which later waits do not
+// sleep any more: the loops run out, the CTA reports and leaves.
+constexpr int kWaitTests = 200000;
+__device__ __forceinline__ void wait_phase(uint64_t *bar, uint32_t parity, int *abort) {
+  if (tc::mbar_try_wait(bar, parity)) return;
   uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(tc::smem_u32(bar)), "r"(parity), "r"(10000u)
-      : "memory");
-  return ok != 0;
+  for (int left = *(volatile int *)abort ? 1 : kWaitTests; left > 0; left--) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(tc::smem_u32(bar)), "r"(parity), "r"(10000u)
+        : "memory");
+    if (ok) return;
+  }
+  *(volatile int *)abort = 1;
 }
 
 }  // namespace kv

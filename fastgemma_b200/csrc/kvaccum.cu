@@ -88,18 +88,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   __syncthreads();
 
-  auto wait = [&](uint64_t *w, uint32_t parity) {
-    if (tc::mbar_try_wait(w, parity)) return;
-    const uint64_t start = tc::globaltimer_ns();
-    while (!mbar_sleep(w, parity)) {
-      if (*(volatile int *)&s_abort) return;
-      if (tc::globaltimer_ns() - start > 2000000000ull) {
-        *(volatile int *)&s_abort = 1;
-        if (ap.err) atomicExch(ap.err, 1);
-        return;
-      }
-    }
-  };
+  auto wait = [&](uint64_t *w, uint32_t parity) { wait_phase(w, parity, &s_abort); };
   const int first = max(t0, live);               // first tile with products
   const int kloads = max(0, t1 - first) * kvh_n; // K tiles, one per KV head
   auto load_k = [&](int i) {
@@ -225,14 +214,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float *ca = &s_cst[buf][0][c0], *cz = &s_cst[buf][1][c0];
         const uint64_t k2 = pair2(scale, scale), l2 = pair2(kLog2e, kLog2e);
         uint64_t add = 0;
-        // the nodes of these rows as bits from the first row's node on
-        uint64_t by = 0;
-        int g = 0;
+        // which of these rows see the slot: each node's bit, once per head
+        uint32_t seen = 0;
         if (masked) {
-          const int n = (blk * kTM + c0) / G, w = n >> 6, sh = n & 63;
-          g = blk * kTM + c0 - n * G;
-          by = s_by[in_tile][w] >> sh;
+          int n = (blk * kTM + c0) / G, g = blk * kTM + c0 - n * G;
+          const int w = n >> 6, sh = n & 63;
+          uint64_t by = s_by[in_tile][w] >> sh;
           if (w < 3 && sh) by |= s_by[in_tile][w + 1] << (64 - sh);
+          const uint32_t heads = G >= 32 ? ~0u : (1u << G) - 1;
+          for (int c = -g; c < kQuarter; c += G, by >>= 1)
+            if (by & 1) seen |= c < 0 ? heads >> -c : heads << c;
         }
         tc::tmem_wait_ld();
 #pragma unroll
@@ -254,10 +245,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             e0 = ex2(e0);
             e1 = ex2(e1);
             if (masked) {
-              if (!(by & 1)) e0 = 0.0f;
-              if (++g == G) g = 0, by >>= 1;
-              if (!(by & 1)) e1 = 0.0f;
-              if (++g == G) g = 0, by >>= 1;
+              if (!((seen >> (c + k)) & 1)) e0 = 0.0f;
+              if (!((seen >> (c + k + 1)) & 1)) e1 = 0.0f;
             }
             add = add2(add, pair2(e0, e1));
           }
@@ -310,6 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   __syncthreads();
   if (s_abort) {  // copies that nobody waited for still land in shared memory
+    if (tid == 0 && ap.err) atomicExch(ap.err, 1);
     if (warp == 0 && lane == 0)
       for (int i = max(0, kloads - ap.kbufs); i < kloads; i++)
         tc::mbar_wait(&bar.k_full[i % ap.kbufs], (i / ap.kbufs) & 1);

@@ -2,20 +2,22 @@
 // tcgen05 tensor cores: tiles of 128 query rows (T nodes x G heads of one KV
 // head) by 128 slots.
 //
-// Per tile: the int32 scores Q8 . K8^T (kind::i8, exact) into one of two TMEM
-// buffers; sixteen softmax warps read them (a lane a row, a quarter of the
-// tile's slots each), scale, mask and exponentiate, and write the weights p *
-// vs back over the scores as two f16 halves (22 bits together, as in the
-// streaming kernel); those are the A operand, from TMEM, of two products with
-// V (kind::f16) that add into the f32 output in TMEM.  V comes from the cache
+// Per tile: the int32 scores Q8 . K8^T (kind::i8, exact) go to TMEM; sixteen
+// softmax warps read them (a lane a row, a quarter of the tile's slots each),
+// which frees the columns for the next tile's, scale, mask and exponentiate,
+// and write the weights p * vs to TMEM as two f16 parts (22 bits together, as
+// in the streaming kernel), 64 slots a buffer; those are the A operand of two
+// products with V (kind::f16) that add into the f32 output in TMEM.  So no
+// MMA is waited for before the next is issued, only their inputs are.  V comes from the cache
 // as int8, four slots of a dimension per word; four warps load it and write
 // the f16 B operand (exact), 64 slots at a time.  The output is rescaled only
 // when a row's maximum has grown by more than 2^8: until then the weights just
 // grow, for which the f16 scale leaves room.
 //
 // The queries are quantised once, by a kernel before, into the swizzled blocks
-// that the tiles copy; partial results of items split over CTAs are joined by
-// one after.
+// that the tiles copy (each CTA for itself took 6 us more at chunk_256_16k: nine
+// CTAs then read the same 128 KB); partial results of items split over CTAs
+// are joined by a kernel after.
 //
 // Bound by the tensor cores: a tile costs 128 * 128 * hd MACs at the int8 rate
 // and twice that at the f16 rate.  Shared memory is next: both operands of the
@@ -37,7 +39,8 @@ constexpr int kThreads = 128 + kSoft + 128;  // loads and MMAs, softmax, V conve
 constexpr int kQuarter = kTN / 4;  // slots of a softmax thread
 constexpr int kGrow = 8;          // log2 by which a row's maximum may grow unnoticed
 constexpr int kUnit = 5;          // f16 weights: p * vs * 2^(kUnit - ve), at most 2^(kUnit + kGrow)
-constexpr uint32_t kColS = 256;   // TMEM columns: output [0, 256), scores / weights 2 x 128
+// TMEM columns: output [0, 256), scores 128, weights of 64 slots 2 x (32 high, 32 low parts)
+constexpr uint32_t kColS = 256, kColP = 384;
 
 struct TileParams {
   TreeParams t;
@@ -53,8 +56,8 @@ struct TileParams {
 };
 
 struct Bars {
-  uint64_t q_full, k_full[4], k_empty[4], v_full[kVStages], v_empty[kVStages], s_full[2], p_full[2],
-      sc_full[2], pv_done;
+  uint64_t q_full, k_full[4], k_empty[4], v_full[kVStages], v_empty[kVStages], s_full, s_empty,
+      p_full[2], p_empty[2], sc_full[2], sc_empty[2];
 };
 
 // SMALL: head_dim <= 256, so that |q8 . k8| < 2^22.
@@ -68,7 +71,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ int s_pos[FGM_CUDA_TREE_MAX], s_low[kTM];
   __shared__ uint64_t s_see[kTM][4];  // nodes each row sees
   __shared__ uint32_t s_tmem;
-  __shared__ int s_abort, s_ve;
+  __shared__ int s_abort, s_top[kThreads / 32];
   const TreeParams &p = tp.t;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int hd = p.kv.head_dim, kvd = p.kv.kv_heads * hd, G = p.n_heads / p.kv.kv_heads;
@@ -87,6 +90,30 @@ __global__ void __launch_bounds__(kThreads, 1)
   const float *ks = p.kv.ks + (size_t)b * p.kv.ks_stride;
   const float *vs = p.kv.vs + (size_t)b * p.kv.vs_stride;
 
+  const int chunks = tiles * tp.nkb, halves = tiles * 2;
+  auto load_k = [&](int c) {  // chunk c: tile c / nkb, bytes 128 * (c % nkb) of the rows
+    const int st = c % tp.kstages, t = c / tp.nkb;
+    tc::mbar_expect_tx(&bar.k_full[st], kChunk);
+    tc::tma_load_3d(ksm + st * kChunk, &kmap, &bar.k_full[st],
+                    kvh * hd + (c - t * tp.nkb) * 128, x0 + t * kTN, b);
+  };
+  auto wait = [&](uint64_t *w, uint32_t parity) { wait_phase(w, parity, &s_abort); };
+
+  // the largest |vs| of the run: the unit of the f16 weights
+  auto exponent = [&](int x) {
+    if (x >= x1 || pos_of(ring, x, end) < 0) return -100;
+    const float v = fabsf(vs[x]);
+    if (!(v > 0.0f && v < INFINITY)) return -100;
+    return max(-100, min((int)((__float_as_uint(v) >> 23) & 255) - 126, 126));
+  };
+  int top_e = -100;
+#pragma unroll 2
+  for (int x = x0 + tid; x < x1; x += kThreads) top_e = max(top_e, exponent(x));
+  int low_pos = 0;
+  if (tid < kTM) {
+    const int node = min(row0 + tid, R - 1) / G;
+    low_pos = p.pos ? p.pos[b * p.T + node] : len + node;
+  }
   if (tid == 0) {
     for (int i = 0; i < 4; i++) {
       tc::mbar_init(&bar.k_full[i], 1);
@@ -97,16 +124,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::mbar_init(&bar.v_empty[i], 1);
     }
     for (int i = 0; i < 2; i++) {
-      tc::mbar_init(&bar.s_full[i], 1);
-      tc::mbar_init(&bar.p_full[i], kSoft);
+      tc::mbar_init(&bar.p_full[i], kSoft / 2);
+      tc::mbar_init(&bar.p_empty[i], 1);
       tc::mbar_init(&bar.sc_full[i], 32);
+      tc::mbar_init(&bar.sc_empty[i], kSoftWarps);
     }
     tc::mbar_init(&bar.q_full, 1);
-    tc::mbar_init(&bar.pv_done, 1);
+    tc::mbar_init(&bar.s_full, 1);
+    tc::mbar_init(&bar.s_empty, kSoftWarps);
     tc::fence_mbar_init();
     s_abort = 0;
-    s_ve = -100;
-    tc::prefetch_tmap(&kmap);
+    for (int c = 0; c < min(chunks, tp.kstages); c++) load_k(c);
     if (wk.t0 == 0) tp.desc[b * p.kv.kv_heads * tp.blocks * tp.dsplit + wk.in_b] =
         make_int2(wk.first, wk.count);
   }
@@ -114,55 +142,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc::tmem_alloc(&s_tmem, 512);
     tc::tmem_relinquish();
   }
-  __syncthreads();
-
-  // A wait that gives up raises the abort word; from then on every wait
-  // returns at once, the loops run out and the CTA leaves.
-  auto wait = [&](uint64_t *w, uint32_t parity) {
-    if (tc::mbar_try_wait(w, parity)) return;
-    const uint64_t t0 = tc::globaltimer_ns();
-    while (!mbar_sleep(w, parity)) {
-      if (*(volatile int *)&s_abort) return;
-      if (tc::globaltimer_ns() - t0 > 2000000000ull) {
-        *(volatile int *)&s_abort = 1;
-        if (tp.err) atomicExch(tp.err, 1);
-        return;
-      }
-    }
-  };
-
-  // first K stages on their way (their barriers are fresh)
-  auto load_k = [&](int c) {  // chunk c: tile c / nkb, bytes 128 * (c % nkb) of the rows
-    const int st = c % tp.kstages, t = c / tp.nkb;
-    tc::mbar_expect_tx(&bar.k_full[st], kChunk);
-    tc::tma_load_3d(ksm + st * kChunk, &kmap, &bar.k_full[st],
-                    kvh * hd + (c - t * tp.nkb) * 128, x0 + t * kTN, b);
-  };
-  const int chunks = tiles * tp.nkb, halves = tiles * 2;
-  if (warp == 0 && lane == 0)
-    for (int c = 0; c < min(chunks, tp.kstages); c++) load_k(c);
-
-  // the largest |vs| of the run: the unit of the f16 weights
-  auto exponent = [&](int x) {
-    if (x >= x1 || pos_of(ring, x, end) < 0) return -100;
-    const float v = fabsf(vs[x]);
-    if (!(v > 0.0f && v < INFINITY)) return -100;
-    return max(-100, min((int)((__float_as_uint(v) >> 23) & 255) - 126, 126));
-  };
-  int top_e = -100;
-  for (int x = x0 + tid; x < x1; x += kThreads) top_e = max(top_e, exponent(x));
   top_e = __reduce_max_sync(0xffffffffu, top_e);
-  if (lane == 0) atomicMax(&s_ve, top_e);
-  if (tid < kTM) {
-    const int node = (row0 + tid) / G;
-    s_low[tid] = tid < rows ? lowest(p.pos ? p.pos[b * p.T + node] : len + node, p.window) : INT_MIN;
-  }
+  if (lane == 0) s_top[warp] = top_e;
+  if (tid < kTM) s_low[tid] = tid < rows ? lowest(low_pos, p.window) : INT_MIN;
   if (p.window)
     for (int i = tid; i < p.T; i += kThreads) s_pos[i] = p.pos ? p.pos[b * p.T + i] : len + i;
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = s_tmem;
+  const int ve = __reduce_max_sync(0xffffffffu, lane < kThreads / 32 ? s_top[lane] : -100);
   const size_t qblock = ((size_t)b * p.kv.kv_heads + kvh) * tp.blocks + blk;
 
   if (warp == 0) {  // ---- the queries, K chunks
@@ -178,7 +167,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp == 2) {  // ---- scales of the slots, two tiles ahead
-    const float unit = pow2(kUnit - s_ve);
+    const float unit = pow2(kUnit - ve);
     for (int j = 0; j < tiles; j++) {
       float a[4], c[4];
 #pragma unroll
@@ -187,7 +176,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         a[k] = x < x1 ? ks[x] : 0.0f;
         c[k] = x < x1 ? vs[x] * unit : 0.0f;
       }
-      if (j >= 2) wait(&bar.p_full[j & 1], ((j - 2) >> 1) & 1);
+      if (j >= 2) wait(&bar.sc_empty[j & 1], ((j - 2) >> 1) & 1);
 #pragma unroll
       for (int k = 0; k < 4; k++) {
         s_ks[j & 1][lane + 32 * k] = a[k];
@@ -203,8 +192,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t id_s = tc::idesc_i8(kTM, kTN), id_o = idesc_f16(kTM, dv);
       int kst = 0, vst = 0;
       uint32_t kph = 0, vph = 0;
-      auto scores = [&](int j) {
-        const uint32_t d = tmem + kColS + (j & 1) * kTN;
+      auto scores = [&] {
+        const uint32_t d = tmem + kColS;
         for (int kb = 0; kb < tp.nkb; kb++) {
           wait(&bar.k_full[kst], kph);
           tc::fence_after_sync();
@@ -218,31 +207,30 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc::mma_commit(&bar.k_empty[kst]);
           if (++kst == tp.kstages) kst = 0, kph ^= 1;
         }
-        tc::mma_commit(&bar.s_full[j & 1]);
+        tc::mma_commit(&bar.s_full);
       };
       wait(&bar.q_full, 0);
-      scores(0);
-      if (tiles > 1) scores(1);
+      scores();
       for (int j = 0; j < tiles; j++) {
-        const uint32_t pb = tmem + kColS + (j & 1) * kTN;
-        wait(&bar.p_full[j & 1], (j >> 1) & 1);
+        if (j + 1 < tiles) {  // the next scores once these are in registers
+          wait(&bar.s_empty, j & 1);
+          scores();
+        }
 #pragma unroll
         for (int h = 0; h < 2; h++) {
+          wait(&bar.p_full[h], j & 1);
           wait(&bar.v_full[vst], vph);
           tc::fence_after_sync();
           const uint64_t v = vd + vst * (dv * 8);
+          const uint32_t a = tmem + kColP + h * 64;
 #pragma unroll
           for (int k = 0; k < 4; k++) {
-            mma_f16_ts(tmem, pb + (h * 4 + k) * 8, v + k * 2, id_o, j + h + k > 0);
-            mma_f16_ts(tmem, pb + 64 + (h * 4 + k) * 8, v + k * 2, id_o, 1);
+            mma_f16_ts(tmem, a + k * 8, v + k * 2, id_o, j + h + k > 0);
+            mma_f16_ts(tmem, a + 32 + k * 8, v + k * 2, id_o, 1);
           }
           tc::mma_commit(&bar.v_empty[vst]);
+          tc::mma_commit(&bar.p_empty[h]);
           if (++vst == kVStages) vst = 0, vph ^= 1;
-        }
-        tc::mma_commit(&bar.pv_done);
-        if (j + 2 < tiles) {  // the weights' columns take new scores once they are read
-          wait(&bar.pv_done, j & 1);
-          scores(j + 2);
         }
       }
     }
@@ -332,10 +320,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto tile = [&](int j, auto is_masked) {
       constexpr bool masked = decltype(is_masked)::value;
       const int buf = j & 1;
-      const uint32_t sc = quad + kColS + buf * kTN;
       const float *ksq = s_ks[buf] + quarter * kQuarter, *vsq = s_vs[buf] + quarter * kQuarter;
       uint32_t s[kQuarter];
-      tc::tmem_ld_x32(sc + quarter * kQuarter, s);
+      tc::tmem_ld_x32(quad + kColS + quarter * kQuarter, s);
       uint32_t seen = 0;
       if (masked) {
         const int x = x0 + j * kTN + quarter * kQuarter, cut = turn - x;
@@ -348,6 +335,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (node < 0) seen = 0;
       }
       tc::tmem_wait_ld();
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&bar.s_empty);
       float top = -INFINITY;
 #pragma unroll
       for (int c = 0; c < kQuarter; c += 4) {
@@ -383,7 +373,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         l *= f;
       }
       if (__any_sync(0xffffffffu, f != 1.0f)) {
-        wait(&bar.pv_done, (j - 1) & 1);
+        wait(&bar.p_empty[0], (j - 1) & 1);
+        wait(&bar.p_empty[1], (j - 1) & 1);
         tc::fence_after_sync();
         for (int c = quarter * (dv / 4); c < (quarter + 1) * (dv / 4); c += 8) {
           uint32_t o[8];
@@ -398,78 +389,93 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float ref = m == -INFINITY ? 0.0f : m;
       const uint64_t qs2 = pair2(qs, qs), ref2 = pair2(-ref, -ref), minus = pair2(-1.0f, -1.0f);
       uint64_t sum = 0;
+      uint32_t hi[16], lo[16];
 #pragma unroll
-      for (int c0 = 0; c0 < kQuarter; c0 += 16) {
-        uint32_t hi[8], lo[8];
+      for (int c = 0; c < kQuarter; c += 4) {
+        const ulonglong2 v4 = *reinterpret_cast<const ulonglong2 *>(vsq + c);
+        const uint64_t vv[2] = {v4.x, v4.y};
 #pragma unroll
-        for (int c = 0; c < 16; c += 4) {
-          const ulonglong2 v4 = *reinterpret_cast<const ulonglong2 *>(vsq + c0 + c);
-          const uint64_t vv[2] = {v4.x, v4.y};
-#pragma unroll
-          for (int k = 0; k < 4; k += 2) {
-            const int i = c0 + c + k;
-            float e0, e1, w0, w1;
-            split2(fma2(pair2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), qs2, ref2), e0, e1);
-            const uint64_t e = pair2(ex2(e0), ex2(e1));
-            sum = add2(sum, e);
-            uint64_t w = mul2(e, vv[k >> 1]);
-            split2(w, w0, w1);
-            if (masked) {  // an unseen slot's scale may be anything
-              if (!((seen >> i) & 1)) w0 = 0.0f;
-              if (!((seen >> (i + 1)) & 1)) w1 = 0.0f;
-              w = pair2(w0, w1);
-            }
-            const __half2 h2 = __floats2half2_rn(w0, w1);
-            const float2 hf = __half22float2(h2);
-            hi[(c + k) / 2] = *reinterpret_cast<const uint32_t *>(&h2);
-            split2(fma2(pair2(hf.x, hf.y), minus, w), w0, w1);
-            lo[(c + k) / 2] = pack2(w0, w1);
+        for (int k = 0; k < 4; k += 2) {
+          const int i = c + k;
+          float e0, e1, w0, w1;
+          split2(fma2(pair2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), qs2, ref2), e0, e1);
+          const uint64_t e = pair2(ex2(e0), ex2(e1));
+          sum = add2(sum, e);
+          uint64_t w = mul2(e, vv[k >> 1]);
+          split2(w, w0, w1);
+          if (masked) {  // an unseen slot's scale may be anything
+            if (!((seen >> i) & 1)) w0 = 0.0f;
+            if (!((seen >> (i + 1)) & 1)) w1 = 0.0f;
+            w = pair2(w0, w1);
           }
+          const __half2 h2 = __floats2half2_rn(w0, w1);
+          const float2 hf = __half22float2(h2);
+          hi[i / 2] = *reinterpret_cast<const uint32_t *>(&h2);
+          split2(fma2(pair2(hf.x, hf.y), minus, w), w0, w1);
+          lo[i / 2] = pack2(w0, w1);
         }
-        tmem_st_x8(sc + quarter * 16 + c0 / 2, hi);
-        tmem_st_x8(sc + 64 + quarter * 16 + c0 / 2, lo);
       }
       float la, lb;
       split2(sum, la, lb);
       l += la + lb;
+      // the buffer's last weights have to be multiplied
+      if (j > 0) wait(&bar.p_empty[quarter >> 1], (j - 1) & 1);
+      tc::fence_after_sync();
+      const uint32_t to = quad + kColP + (quarter >> 1) * 64 + (quarter & 1) * 16;
+      tmem_st_x16(to, hi);
+      tmem_st_x16(to + 32, lo);
       tmem_wait_st();
     };
     for (int j = 0; j < tiles; j++) {
       wait(&bar.sc_full[j & 1], (j >> 1) & 1);
-      wait(&bar.s_full[j & 1], (j >> 1) & 1);
+      wait(&bar.s_full, j & 1);
       tc::fence_after_sync();
-      if (idle) meet();
-      else if (ring || x0 + (j + 1) * kTN > len || x0 + j * kTN < high)
+      if (idle) {
+        if (lane == 0) tc::mbar_arrive(&bar.s_empty);
+        if (j > 0) wait(&bar.p_empty[quarter >> 1], (j - 1) & 1);
+      } else if (ring || x0 + (j + 1) * kTN > len || x0 + j * kTN < high) {
         tile(j, std::true_type());
-      else
+      } else {
         tile(j, std::false_type());
+      }
       tc::fence_before_sync();
-      tc::mbar_arrive(&bar.p_full[j & 1]);
+      tc::mbar_arrive(&bar.p_full[quarter >> 1]);
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&bar.sc_empty[j & 1]);
     }
     // ---- results: the quarters' sums joined, each quarter's dimensions to
     // shared memory, whole rows from there (what the loads filled is free now)
     s_l[quarter][row] = l;
     meet();
     const float L = (s_l[0][row] + s_l[1][row]) + (s_l[2][row] + s_l[3][row]);
-    wait(&bar.pv_done, (tiles - 1) & 1);
+    wait(&bar.p_empty[0], (tiles - 1) & 1);
+    wait(&bar.p_empty[1], (tiles - 1) & 1);
     tc::fence_after_sync();
     const bool whole = wk.count == 1;
-    float back = pow2(s_ve) * 0.03125f;  // 2^-kUnit
+    float back = pow2(ve) * 0.03125f;  // 2^-kUnit
     if (whole) back = L == 0.0f ? 0.0f : back / L;
     float *stage = reinterpret_cast<float *>(sm + (size_t)row * (dv * 4 + 16));
-    if (!idle)  // column e * dv / 4 + i of the output is dimension 4 i + e
-#pragma unroll 4
-      for (int i = quarter * (dv / 16); i < (quarter + 1) * (dv / 16); i += 2) {
-        uint32_t o[4][2];
+    // column e * dv / 4 + i of the output is dimension 4 i + e
+    auto put = [&](auto step) {
+      constexpr int N = decltype(step)::value;
+      for (int i = quarter * (dv / 16); i < (quarter + 1) * (dv / 16); i += N) {
+        uint32_t o[4][N];
 #pragma unroll
-        for (int e = 0; e < 4; e++) tmem_ld_x2(quad + e * (dv / 4) + i, o[e]);
+        for (int e = 0; e < 4; e++) tmem_ld<N>(quad + e * (dv / 4) + i, o[e]);
         tc::tmem_wait_ld();
 #pragma unroll
-        for (int k = 0; k < 2; k++)
+        for (int k = 0; k < N; k++)
           *reinterpret_cast<float4 *>(stage + 4 * (i + k)) =
               make_float4(__uint_as_float(o[0][k]) * back, __uint_as_float(o[1][k]) * back,
                           __uint_as_float(o[2][k]) * back, __uint_as_float(o[3][k]) * back);
       }
+    };
+    if (idle) {
+    } else if (dv % 128 == 0) {
+      put(std::integral_constant<int, 8>());
+    } else {
+      put(std::integral_constant<int, 2>());
+    }
     tc::fence_before_sync();
     stream::fence_proxy_async_smem();
     meet();
@@ -487,6 +493,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   __syncthreads();
   if (s_abort) {  // copies that nobody waited for still land in shared memory
+    if (tid == 0 && tp.err) atomicExch(tp.err, 1);
     if (warp == 0 && lane == 0)
       for (int c = max(0, chunks - tp.kstages); c < chunks; c++)
         tc::mbar_wait(&bar.k_full[c % tp.kstages], (c / tp.kstages) & 1);
@@ -523,23 +530,24 @@ __global__ void __launch_bounds__(kJoin) tile_join_kernel(const __grid_constant_
   const float4 *part = reinterpret_cast<const float4 *>(tp.part) + ((size_t)de.x * kTM + row) * dv4 + d;
   float M = -INFINITY, L = 0.0f;
   float4 a = make_float4(0, 0, 0, 0);
-  for (int i0 = 0; i0 < de.y; i0 += 8) {
-    float2 s[8];
-    float4 v[8];
-    const int n = min(8, de.y - i0);
+  constexpr int kParts = 12;
+  for (int i0 = 0; i0 < de.y; i0 += kParts) {
+    float2 s[kParts];
+    float4 v[kParts];
+    const int n = min(kParts, de.y - i0);
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
+    for (int i = 0; i < kParts; i++) {
       s[i] = i < n ? stat[(size_t)(i0 + i) * kTM] : make_float2(-INFINITY, 0.0f);
       v[i] = i < n ? part[(size_t)(i0 + i) * kTM * dv4] : make_float4(0, 0, 0, 0);
     }
     float N = M;
 #pragma unroll
-    for (int i = 0; i < 8; i++) N = fmaxf(N, s[i].x);
+    for (int i = 0; i < kParts; i++) N = fmaxf(N, s[i].x);
     const float ref = N == -INFINITY ? 0.0f : N, f0 = ex2(M - ref);
     a.x *= f0, a.y *= f0, a.z *= f0, a.w *= f0;
     L *= f0;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
+    for (int i = 0; i < kParts; i++) {
       const float f = ex2(s[i].x - ref);
       L += f * s[i].y;
       a.x += f * v[i].x, a.y += f * v[i].y, a.z += f * v[i].z, a.w += f * v[i].w;

@@ -4,6 +4,7 @@
 #pragma once
 
 #include <atomic>
+#include <type_traits>
 
 #include <cuda_fp16.h>
 
@@ -102,6 +103,15 @@ __device__ __forceinline__ int tiles_of(const Span &s, int tile) {
   return (s.end - s.first + tile - 1) / tile;
 }
 
+// x / d for x >= 0, d > 0: by f32 where both are exact there, which takes a
+// fifth of the integer division's time at the head of every CTA.
+__device__ __forceinline__ int quick_div(int x, int d) {
+  if (x >= (1 << 22) || d >= (1 << 22)) return x / d;
+  int q = (int)__fdividef((float)x, (float)d);
+  const int r = x - q * d;
+  return r < 0 ? q - 1 : (r >= d ? q + 1 : q);
+}
+
 template <bool ALL = false>
 __device__ __forceinline__ bool find_work(const TreeParams &p, int tile, int per_b, int min_per,
                                           int lane, Work &w) {
@@ -111,19 +121,19 @@ __device__ __forceinline__ bool find_work(const TreeParams &p, int tile, int per
   int total = n0;
   for (int b = lane + 32; b < rows; b += 32) total += tiles_of(span_of<ALL>(p, b), tile);
   total = __reduce_add_sync(0xffffffffu, total);
-  const long long units = (long long)total * per_b;
-  int per = max(min_per, (int)((units + grid - 1) / grid));
+  // from just below the even share upwards
+  int per = max(min_per, (int)(__fdividef((float)total * (float)per_b, (float)grid) * 0.9999f));
   for (;; per += 1 + per / 32) {
-    int c = (n0 + per - 1) / per;
+    int c = quick_div(n0 + per - 1, per);
     for (int b = lane + 32; b < rows; b += 32)
       c += (tiles_of(span_of<ALL>(p, b), tile) + per - 1) / per;
-    if (__reduce_add_sync(0xffffffffu, c) * per_b <= grid) break;
+    if ((long long)__reduce_add_sync(0xffffffffu, c) * per_b <= grid) break;
   }
   int base = 0;
   for (int b0 = 0; b0 < rows; b0 += 32) {
     const int b = b0 + lane;
     const Span s = b0 == 0 ? mine : span_of<ALL>(p, min(b, rows - 1));
-    const int tiles = b < rows ? tiles_of(s, tile) : 0, cnt = (tiles + per - 1) / per;
+    const int tiles = b < rows ? tiles_of(s, tile) : 0, cnt = quick_div(tiles + per - 1, per);
     int inc = cnt * per_b;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -140,8 +150,8 @@ __device__ __forceinline__ bool find_work(const TreeParams &p, int tile, int per
       w.b = b0 + l;
       w.count = __shfl_sync(0xffffffffu, cnt, l);
       const int rel = cta - base - __shfl_sync(0xffffffffu, inc - cnt * per_b, l);
-      w.in_b = rel / w.count;
-      const int k = rel - w.in_b * w.count, each = t / w.count, more = t - each * w.count;
+      w.in_b = quick_div(rel, w.count);
+      const int k = rel - w.in_b * w.count, each = quick_div(t, w.count), more = t - each * w.count;
       w.first = cta - k;
       w.t0 = k * each + min(k, more);
       w.t1 = w.t0 + each + (k < more);
@@ -163,7 +173,7 @@ struct Parts {
 
 __device__ __forceinline__ void store_row4(const TreeParams &p, const Work &w, int kvh, int r,
                                            int d, float4 a, float M, float L) {
-  const int hd = p.kv.head_dim, G = p.n_heads / p.kv.kv_heads, node = r / G;
+  const int hd = p.kv.head_dim, G = p.n_heads / p.kv.kv_heads, node = quick_div(r, G);
   const int h = kvh * G + r - node * G;
   const size_t qr = (size_t)w.b * p.T + node;
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
@@ -175,61 +185,82 @@ __device__ __forceinline__ void store_row4(const TreeParams &p, const Work &w, i
 
 // Every thread of the CTA, after its partial results are written.  sm: at
 // least rows * (count + 2) floats of shared memory that nothing else uses.
+// The barrier orders the CTA's stores before thread 0's fence, the fence them
+// before its count; whoever counts last reads what all the others wrote.
 __device__ __forceinline__ void join_parts(const TreeParams &p, const Parts &q, const Work &w,
                                            int kvh, int row0, int rows, int ld, float *sm) {
   __shared__ int s_last;
   const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31;
-  __threadfence();
   __syncthreads();
   if (tid == 0) {
+    __threadfence();
     s_last = atomicAdd(q.counters + w.first, 1) == w.count - 1;
     if (s_last) q.counters[w.first] = 0;
+    __threadfence();
   }
   __syncthreads();
   if (!s_last) return;
-  __threadfence();
-  const int n = w.count, hd4 = p.kv.head_dim / 4;
+  const int n = w.count, hd4 = p.kv.head_dim / 4, total = rows * hd4;
   float *f = sm, *tot = sm + rows * n;
   const float2 *stat = q.stat + (size_t)w.first * ld;
-  for (int r = tid >> 5; r < rows; r += nt >> 5) {
+  for (int r = tid >> 5; r < rows; r += nt >> 5) {  // a warp per row: the parts' factors
     float M = -INFINITY, L = 0.0f;
-    for (int i = lane; i < n; i += 32) M = fmaxf(M, __ldcg(&stat[(size_t)i * ld + r].x));
-    M = warp_max(M);
-    const float ref = M == -INFINITY ? 0.0f : M;
-    for (int i = lane; i < n; i += 32) {
-      const float2 v = __ldcg(&stat[(size_t)i * ld + r]);
-      const float e = ex2(v.x - ref);
-      f[r * n + i] = e;
-      L += e * v.y;
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      const float2 v = i0 + lane < n ? __ldcg(&stat[(size_t)(i0 + lane) * ld + r])
+                                     : make_float2(-INFINITY, 0.0f);
+      const float N = fmaxf(M, warp_max(v.x)), ref = N == -INFINITY ? 0.0f : N;
+      L = L * ex2(M - ref) + v.y * ex2(v.x - ref);
+      M = N;
+      if (i0 + lane < n) f[r * n + i0 + lane] = v.x;
     }
+    const float ref = M == -INFINITY ? 0.0f : M;
+    for (int i = lane; i < n; i += 32) f[r * n + i] = ex2(f[r * n + i] - ref);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
     if (lane == 0) tot[2 * r] = M, tot[2 * r + 1] = L;
   }
   __syncthreads();
-  for (int i = tid; i < rows * hd4; i += nt) {
-    const int r = i / hd4, d = i - r * hd4;
-    const float4 *src = reinterpret_cast<const float4 *>(q.part) +
-                        ((size_t)w.first * ld + r) * hd4 + d;
-    float4 a = make_float4(0, 0, 0, 0);
-    int k = 0;
-    for (; k + 8 <= n; k += 8) {
-      float4 v[8];
+  // U outputs of a thread at a time, P parts of each on their way together
+  const float4 *part = reinterpret_cast<const float4 *>(q.part) + (size_t)w.first * ld * hd4;
+  auto join = [&](auto us, auto ps) {
+    constexpr int U = decltype(us)::value, P = decltype(ps)::value;
+    for (int i0 = tid; i0 < total; i0 += nt * U) {
+      float4 a[U];
 #pragma unroll
-      for (int u = 0; u < 8; u++) v[u] = __ldcg(src + (size_t)(k + u) * ld * hd4);
+      for (int u = 0; u < U; u++) a[u] = make_float4(0, 0, 0, 0);
+      for (int k = 0; k < n; k += P) {
+        float4 v[U][P];
 #pragma unroll
-      for (int u = 0; u < 8; u++) {
-        const float e = f[r * n + k + u];
-        a.x += e * v[u].x, a.y += e * v[u].y, a.z += e * v[u].z, a.w += e * v[u].w;
+        for (int u = 0; u < U; u++)
+#pragma unroll
+          for (int e = 0; e < P; e++)
+            v[u][e] = i0 + u * nt < total && k + e < n
+                          ? __ldcg(part + (size_t)(k + e) * ld * hd4 + i0 + u * nt)
+                          : make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+          const float *fr = f + quick_div(min(i0 + u * nt, total - 1), hd4) * n + k;
+#pragma unroll
+          for (int e = 0; e < P; e++)
+            if (k + e < n) {
+              const float s = fr[e];
+              a[u].x += s * v[u][e].x, a[u].y += s * v[u][e].y;
+              a[u].z += s * v[u][e].z, a[u].w += s * v[u][e].w;
+            }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const int i = i0 + u * nt;
+        if (i < total) {
+          const int r = quick_div(i, hd4);
+          store_row4(p, w, kvh, row0 + r, (i - r * hd4) * 4, a[u], tot[2 * r], tot[2 * r + 1]);
+        }
       }
     }
-    for (; k < n; k++) {
-      const float4 v = __ldcg(src + (size_t)k * ld * hd4);
-      const float e = f[r * n + k];
-      a.x += e * v.x, a.y += e * v.y, a.z += e * v.z, a.w += e * v.w;
-    }
-    store_row4(p, w, kvh, row0 + r, d * 4, a, tot[2 * r], tot[2 * r + 1]);
-  }
+  };
+  if (total <= nt) join(std::integral_constant<int, 1>(), std::integral_constant<int, 12>());
+  else join(std::integral_constant<int, 4>(), std::integral_constant<int, 4>());
 }
 
 // ------------------------------------------------------------------ host side

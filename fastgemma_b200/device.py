@@ -10,7 +10,7 @@ import ctypes as C
 
 import torch
 
-from ._lib import call
+from ._lib import FgmCudaError, call, lib
 
 
 def _s(stream):
@@ -279,6 +279,8 @@ def attend_workspace(kv, n_heads, T):
     """A workspace for the attention entries on this cache, zeroed as its first
     use needs it; to be kept from call to call, by one stream at a time."""
     n = call("fgm_cuda_attend_workspace", C.byref(kv), n_heads, T)
+    if n == 0 and kv.rows:
+        raise FgmCudaError(-1, lib().fgm_cuda_last_error().decode())
     return torch.zeros(max(int(n), 1), dtype=torch.uint8, device="cuda")
 
 

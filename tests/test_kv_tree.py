@@ -817,3 +817,28 @@ def test_views_check_their_tensors():
         D.KvCache(kc, s, vt, s, 1, 64, acc=torch.zeros(2, 7))
     with pytest.raises(ValueError, match="mask has to be contiguous"):
         D._flat(lens=None, mask=torch.zeros(4, 4).t())
+
+
+# ------------------------------------------------------------- all together
+@gpu
+def test_speculative_decoding_gives_the_tokens_of_single_steps():
+    """The example: the same greedy tokens in fewer steps, and a cache held to
+    its budget goes on generating."""
+    import os
+    import sys
+    sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "examples"))
+    import speculative_decode as S
+    first = torch.tensor([3, 77], dtype=torch.int32, device="cuda")
+    n = 48
+    plain = S.generate(S.Model(2, n + 32), first, n).tolist()
+    spec, steps = S.speculate(S.Model(2, n + 32), first, n, 8)
+    assert [s[:n] for s in spec] == plain
+    assert steps < n
+    model = S.Model(2, 64)
+    held, _ = S.speculate(model, first, n, 8, budget=24)
+    assert all(len(h) >= n for h in held) and int(model.lens.max()) <= 24 + 8
+    for kv in model.caches:  # the first tokens and the newest are still there
+        tpos = kv._keep[5].cpu().numpy()
+        for b, m in enumerate(model.lens.tolist()):
+            assert set(range(4)) <= set(tpos[b, :m].tolist())
+            assert len(set(tpos[b, :m].tolist())) == m

@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ uint64_t s_see[FGM_CUDA_TREE_MAX][4];  // nodes that each node sees
   __shared__ uint64_t s_by[kTN][4];                 // nodes that see each slot of a tile
   __shared__ uint32_t s_tmem;
-  __shared__ int s_abort, s_high;
+  __shared__ int s_abort, s_high[kThreads / 32];
   const TreeParams &p = ap.t;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int hd = p.kv.head_dim, G = p.n_heads / p.kv.kv_heads, R = p.T * G, kvh_n = p.kv.kv_heads;
@@ -63,6 +63,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   // tiles below this hold no slot that a node sees: they only decay
   const int live = ring ? 0 : span_of(p, b).first / kTN;
 
+  const int first = max(t0, live);               // first tile with products
+  const int kloads = max(0, t1 - first) * kvh_n; // K tiles, one per KV head
+  auto load_k = [&](int i) {
+    const int buf = i % ap.kbufs, t = first + i / kvh_n, kvh = i % kvh_n;
+    tc::mbar_expect_tx(&bar.k_full[buf], (uint32_t)ap.nkb * kChunk);
+    for (int kb = 0; kb < ap.nkb; kb++)
+      tc::tma_load_3d(ksm + (buf * ap.nkb + kb) * kChunk, &kmap, &bar.k_full[buf],
+                      kvh * hd + kb * 128, t * kTN, b);
+  };
+  auto wait = [&](uint64_t *w, uint32_t parity) { wait_phase(w, parity, &s_abort); };
   if (tid == 0) {
     for (int i = 0; i < 2; i++) {
       tc::mbar_init(&bar.k_full[i], 1);
@@ -79,29 +89,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     tc::fence_mbar_init();
     s_abort = 0;
-    s_high = INT_MIN;
-    tc::prefetch_tmap(&kmap);
+    for (int i = 0; i < min(kloads, ap.kbufs); i++) load_k(i);
   }
   if (warp == 1) {
     tc::tmem_alloc(&s_tmem, 512);
     tc::tmem_relinquish();
   }
-  __syncthreads();
-
-  auto wait = [&](uint64_t *w, uint32_t parity) { wait_phase(w, parity, &s_abort); };
-  const int first = max(t0, live);               // first tile with products
-  const int kloads = max(0, t1 - first) * kvh_n; // K tiles, one per KV head
-  auto load_k = [&](int i) {
-    const int buf = i % ap.kbufs, t = first + i / kvh_n, kvh = i % kvh_n;
-    tc::mbar_expect_tx(&bar.k_full[buf], (uint32_t)ap.nkb * kChunk);
-    for (int kb = 0; kb < ap.nkb; kb++)
-      tc::tma_load_3d(ksm + (buf * ap.nkb + kb) * kChunk, &kmap, &bar.k_full[buf],
-                      kvh * hd + kb * 128, t * kTN, b);
-  };
-  if (warp == 0 && lane == 0)
-    for (int i = 0; i < min(kloads, ap.kbufs); i++) load_k(i);
-
   // what each node sees of the nodes, and its lowest position
+  int high = INT_MIN;
   for (int i = tid; i < p.T * 4; i += kThreads) {
     const int node = i >> 2, w = i & 3;
     const int low = lowest(p.pos ? p.pos[b * p.T + node] : len + node, p.window);
@@ -115,15 +110,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           if ((p.pos ? p.pos[b * p.T + w * 64 + k] : len + w * 64 + k) < low) v &= ~(1ull << k);
     }
     s_see[node][w] = v;
-    if (w == 0) {
-      s_low[node] = low;
-      if (p.window) atomicMax(&s_high, low);
-    }
+    if (w == 0) s_low[node] = low;
+    high = max(high, low);
   }
+  high = __reduce_max_sync(0xffffffffu, high);
+  if (lane == 0) s_high[warp] = high;
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = s_tmem;
+  high = __reduce_max_sync(0xffffffffu, lane < kThreads / 32 ? s_high[lane] : INT_MIN);
   const int units = kloads * ap.blocks;  // score blocks
 
   if (warp == 0) {  // ---- K tiles
@@ -196,7 +192,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t quad = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const float *ks = p.kv.ks + (size_t)b * p.kv.ks_stride;
     float *acc = p.kv.acc + (size_t)b * p.kv.acc_stride;
-    const int high = s_high;
     // the four warps that share the quadrant's slots
     auto meet = [&] { asm volatile("bar.sync %0, 128;" ::"r"(1 + (warp & 3)) : "memory"); };
     int u = 0;
@@ -327,12 +322,12 @@ __global__ void __launch_bounds__(kQuantRows * 32)
     quant_rows_kernel(const __grid_constant__ TreeParams p, int blocks, int nkb, int8_t *q8,
                       float *qs, float *cst) {
   const int lane = threadIdx.x & 31;
-  const long long row = (long long)blockIdx.x * kQuantRows + (threadIdx.x >> 5);
+  const unsigned row = blockIdx.x * kQuantRows + (threadIdx.x >> 5);
   const int hd = p.kv.head_dim, G = p.n_heads / p.kv.kv_heads, R = p.T * G;
   stream::pdl_launch_dependents();
   const int block = (int)(row / kTM), j = (int)(row % kTM);
-  const int bk = block / blocks, r = (block - bk * blocks) * kTM + j;
-  const int b = bk / p.kv.kv_heads, kvh = bk - b * p.kv.kv_heads;
+  const int bk = quick_div(block, blocks), r = (block - bk * blocks) * kTM + j;
+  const int b = quick_div(bk, p.kv.kv_heads), kvh = bk - b * p.kv.kv_heads;
   if (r >= R) {
     if (cst && lane == 0) {
       cst[(size_t)block * 2 * kTM + j] = 0.0f;
@@ -340,7 +335,7 @@ __global__ void __launch_bounds__(kQuantRows * 32)
     }
     return;
   }
-  const int node = r / G, h = kvh * G + r - node * G;
+  const int node = quick_div(r, G), h = kvh * G + r - node * G;
   const size_t qr = (size_t)b * p.T + node;
   const float4 *src = reinterpret_cast<const float4 *>(p.q + qr * p.q_ld + (size_t)h * hd);
   float4 v[4];

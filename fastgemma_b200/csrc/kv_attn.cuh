@@ -86,9 +86,9 @@ __device__ __forceinline__ Span span_of(const TreeParams &p, int b) {
 // ------------------------------------------------------------- the work list
 // Items (sequence, KV head, row block) of `tiles` slot tiles each, one run of
 // an item's tiles per CTA.  Lengths are known on the device only, so every
-// warp finds its CTA's run itself: the fewest tiles per CTA (at least
-// min_per) for which all runs fit the grid, which holds at least one CTA per
-// item.  Splitting items instead of a flat list of tiles costs at most one
+// warp finds its CTA's run itself: the fewest tiles per CTA for which all runs
+// fit the grid, which holds at least one CTA per item; where no item has more
+// than `whole` tiles, one CTA takes each, which spares the join.  Splitting items instead of a flat list of tiles costs at most one
 // tile of balance and saves a CTA from working on two items in turn (5 us).
 constexpr int kCounters = 16384;  // grid of a launch with split items, at most
 
@@ -113,16 +113,22 @@ __device__ __forceinline__ int quick_div(int x, int d) {
 }
 
 template <bool ALL = false>
-__device__ __forceinline__ bool find_work(const TreeParams &p, int tile, int per_b, int min_per,
+__device__ __forceinline__ bool find_work(const TreeParams &p, int tile, int per_b, int whole,
                                           int lane, Work &w) {
   const int rows = p.kv.rows, grid = gridDim.x, cta = blockIdx.x;
   const Span mine = span_of<ALL>(p, min(lane, rows - 1));
   const int n0 = lane < rows ? tiles_of(mine, tile) : 0;  // the first 32 sequences stay here
-  int total = n0;
-  for (int b = lane + 32; b < rows; b += 32) total += tiles_of(span_of<ALL>(p, b), tile);
+  int total = n0, longest = n0;
+  for (int b = lane + 32; b < rows; b += 32) {
+    const int n = tiles_of(span_of<ALL>(p, b), tile);
+    total += n;
+    longest = max(longest, n);
+  }
   total = __reduce_add_sync(0xffffffffu, total);
+  longest = __reduce_max_sync(0xffffffffu, longest);
   // from just below the even share upwards
-  int per = max(min_per, (int)(__fdividef((float)total * (float)per_b, (float)grid) * 0.9999f));
+  int per = max(longest <= whole ? longest : 1,
+                (int)(__fdividef((float)total * (float)per_b, (float)grid) * 0.9999f));
   for (;; per += 1 + per / 32) {
     int c = quick_div(n0 + per - 1, per);
     for (int b = lane + 32; b < rows; b += 32)

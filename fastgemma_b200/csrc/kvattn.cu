@@ -71,6 +71,11 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
 // |vs|), 22 bits in all, so the products lose less than f32 rounding does.
 constexpr int kTile = 128;   // slots per tile of the work list
 constexpr int kStep = 16;    // slots per warp step
+// Tiles of an item that one CTA takes alone: another tile there against the
+// join of two CTAs, measured at two tiles 9.2 against 9.9 us (4 rows, head_dim
+// 256) and 12.8 against 16.3 (16 rows), at four 11.9 against 10.0 and 16.4
+// against 15.8; at four of head_dim 64 8.0 against 8.6 and 10.8 against 11.0.
+__host__ __device__ constexpr int whole_tiles(int hd) { return hd <= 128 ? 4 : 2; }
 
 __host__ __device__ constexpr int stream_warps(int hd) { return hd <= 256 ? 8 : 4; }
 __host__ __device__ constexpr int stage_bytes(int hd) { return 32 * hd + 16 * 16 + 4 * 32 + 128; }
@@ -87,7 +92,6 @@ struct StreamParams {
   TreeParams t;
   Parts parts;
   int blocks;       // row blocks per (sequence, KV head)
-  int min_per;      // tiles per CTA, at least
   float *scores;    // [rows][n_heads][score_ld], or null
   int score_ld;
 };
@@ -108,7 +112,7 @@ __global__ void __launch_bounds__(stream_warps(HD) * 32, 1)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   uint8_t *q8 = sm + W * S * SB;
   Work wk;
-  if (!find_work(p, kTile, p.kv.kv_heads * sp.blocks, sp.min_per, lane, wk)) return;
+  if (!find_work(p, kTile, p.kv.kv_heads * sp.blocks, whole_tiles(HD), lane, wk)) return;
   const int b = wk.b, kvh = wk.in_b / sp.blocks, row0 = (wk.in_b - kvh * sp.blocks) * ROWS;
   const int len = wk.span.len, ring = p.kv.ring, end = len + p.T;
   const int x0 = wk.span.first + wk.t0 * kTile, x1 = min(wk.span.end, wk.span.first + wk.t1 * kTile);
@@ -508,7 +512,6 @@ cudaError_t launch_stream(const TreeParams &p, bool accumulate, int num_sms, cud
   StreamParams sp;
   sp.t = p;
   sp.blocks = blocks;
-  sp.min_per = 1;
   const int grid = grid_of(p.kv, (long long)p.kv.rows * p.kv.kv_heads * blocks, kTile,
                            num_sms < kMaxSms ? num_sms : kMaxSms);
   sp.parts.part = reinterpret_cast<float *>(ws + w.part);
@@ -551,18 +554,31 @@ cudaError_t launch_stream(const TreeParams &p, bool accumulate, int num_sms, cud
 
 }  // namespace
 
-// Up to 16 query rows per KV head the cache's bytes bound the work and the
-// streaming kernel reads them once; from there on its tensor instructions do.
-bool streams(const fgm_cuda_kv &kv, int n_heads, int T) { return T * (n_heads / kv.kv_heads) <= 16; }
+// The streaming kernel up to 16 query rows per KV head, where the cache's bytes
+// bound the work; beyond, the tensor tiles, except over caches so short that
+// the row blocks of 16 fit the SMs at once and run their few slots through
+// before a tile kernel's three launches would be done: at 230 slots of head_dim
+// 256 and 64 rows for each of 8 sequences 12.8 against 17.1 us, at 990 slots
+// 23.5 against 19.1; at 990 of head_dim 64 14.0 against 17.3, at 4000 24.2
+// against 24.0.
+bool streams(const TreeParams &p) {
+  const int R = p.T * (p.n_heads / p.kv.kv_heads);
+  if (R <= 16) return true;
+  long long slots = p.kv.ring ? p.kv.ring : p.kv.cap;
+  if (p.window) slots = std::min(slots, (long long)p.window + p.T + 16);
+  int nt, blocks;
+  stream_blocks(p.kv, p.n_heads, p.T, nt, blocks);
+  return slots <= (p.kv.head_dim <= 128 ? 1024 : 256) &&
+         (long long)p.kv.rows * p.kv.kv_heads * blocks <= 144;
+}
 
 size_t attend_workspace(const fgm_cuda_kv &kv, int n_heads, int T) {
-  const size_t n = streams(kv, n_heads, T) ? ws_of(kv, n_heads, T).total
-                                           : attend_tile_workspace(kv, n_heads, T);
+  const size_t n = std::max(ws_of(kv, n_heads, T).total, attend_tile_workspace(kv, n_heads, T));
   return std::max(n, accum_workspace(kv, n_heads, T));
 }
 
 cudaError_t launch_attend_tree(const TreeParams &p, int num_sms, int *err, cudaStream_t st) {
-  if (!streams(p.kv, p.n_heads, p.T)) return launch_attend_tile(p, num_sms, err, st);
+  if (!streams(p)) return launch_attend_tile(p, num_sms, err, st);
   return launch_stream(p, false, num_sms, st);
 }
 

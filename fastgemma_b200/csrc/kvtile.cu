@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   Work wk;
-  if (!find_work(p, kTN, p.kv.kv_heads * tp.blocks * tp.dsplit, 1, lane, wk)) return;
+  if (!find_work(p, kTN, p.kv.kv_heads * tp.blocks * tp.dsplit, 2, lane, wk)) return;
   const int b = wk.b, ds = wk.in_b % tp.dsplit, blk = wk.in_b / tp.dsplit % tp.blocks;
   const int kvh = wk.in_b / (tp.dsplit * tp.blocks), row0 = blk * kTM, rows = min(kTM, R - row0);
   const int len = wk.span.len, ring = p.kv.ring, end = len + p.T;

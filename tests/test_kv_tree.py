@@ -238,49 +238,59 @@ SHAPES = [
     ([500, 3], 60, 8, 2, 128, "tree", 100, 160),
     ([640, 0], 100, 2, 1, 320, "chain", 29, 131),
     ([10000], 1, 8, 2, 256, "chain", 33, 33),
+    ([2000, 37, 290], 20, 8, 2, 256, "tree", 280, 300),
+    ([3000], 30, 4, 2, 64, "any", 1000, 1100),
+    ([700, 5], 70, 2, 1, 512, "chain", 230, 300),
 ]
+# slots past the nodes: many rows over a cache with room take another kernel
+# than over one that is short
+ROOM = [5, 1200]
 
 
 @gpu
+@pytest.mark.parametrize("room", ROOM)
 @pytest.mark.parametrize("lens,T,H,kvh,hd,kind,window,ring", SHAPES)
-def test_attend_tree(lens, T, H, kvh, hd, kind, window, ring):
+def test_attend_tree(lens, T, H, kvh, hd, kind, window, ring, room):
     rng = np.random.default_rng(sum(lens) * 7 + T * 31 + H + hd)
-    cache, q, mask, pos = setup(rng, lens, T, H, kvh, hd, kind, window, ring)
+    cache, q, mask, pos = setup(rng, lens, T, H, kvh, hd, kind, window, ring, room)
     check_attend(cache, q, H, T, lens, mask, pos, window)
 
 
 @gpu
-@pytest.mark.parametrize("T,H,kvh,hd", [(3, 8, 2, 256), (40, 8, 2, 64)])
-def test_attend_strides_and_flat_or_peaked_scores(T, H, kvh, hd):
+@pytest.mark.parametrize("T,H,kvh,hd,room", [(3, 8, 2, 256, 5), (40, 8, 2, 64, 5),
+                                             (40, 8, 2, 64, 1200), (70, 4, 1, 320, 200)])
+def test_attend_strides_and_flat_or_peaked_scores(T, H, kvh, hd, room):
     """Rows and sequences further apart than they are long; a zero query (all
     weights equal) and one slot that takes all the weight."""
     rng = np.random.default_rng(T)
     lens = [150, 149]
-    cache, q, mask, pos = setup(rng, lens, T, H, kvh, hd)
+    cache, q, mask, pos = setup(rng, lens, T, H, kvh, hd, extra=room)
     q[1] = 0.0
     q[2] *= 40.0
     check_attend(cache, q, H, T, lens, mask, pos, 0, pad=3, q_pad=12)
 
 
 @gpu
-def test_attend_scales_of_every_size():
+@pytest.mark.parametrize("T,room", [(2, 5), (20, 5), (20, 1200)])
+def test_attend_scales_of_every_size(T, room):
     """V scales from 1e-30 to 1e30 and zero, negative K and V scales: the
     weights keep their precision whatever the scales' range."""
     rng = np.random.default_rng(2)
-    lens, T, H, kvh, hd = [300], 2, 8, 2, 128
+    lens, H, kvh, hd = [300], 8, 2, 128
     for lo, hi in ((-30, -28), (28, 30), (-3, 3)):
-        cache, q, mask, pos = setup(rng, lens, T, H, kvh, hd, scale=0.2)
-        cache.vs[:, :302] = (10.0 ** rng.uniform(lo, hi, 302) * rng.choice([1, -1, 0], 302))
+        cache, q, mask, pos = setup(rng, lens, T, H, kvh, hd, scale=0.2, extra=room)
+        n = 300 + T
+        cache.vs[:, :n] = (10.0 ** rng.uniform(lo, hi, n) * rng.choice([1, -1, 0], n))
         cache.ks[:, ::2] *= -1
         check_attend(cache, q, H, T, lens, mask, pos, 0)
 
 
 @gpu
-@pytest.mark.parametrize("T,hd", [(2, 128), (48, 256)])
-def test_a_query_that_is_no_number_stays_in_its_head(T, hd):
+@pytest.mark.parametrize("T,hd,room", [(2, 128, 5), (48, 256, 5), (48, 256, 300), (48, 64, 1200)])
+def test_a_query_that_is_no_number_stays_in_its_head(T, hd, room):
     rng = np.random.default_rng(5)
     H, kvh, lens = 4, 2, [70]
-    cache, q, mask, pos = setup(rng, lens, T, H, kvh, hd)
+    cache, q, mask, pos = setup(rng, lens, T, H, kvh, hd, extra=room)
     want = run_attend(cache, q, H, T, lens, mask, pos, 0)
     q[1, hd + 3] = np.nan
     q[0, 2 * hd] = np.inf
@@ -294,10 +304,10 @@ def test_a_query_that_is_no_number_stays_in_its_head(T, hd):
 
 
 @gpu
-@pytest.mark.parametrize("T", [1, 40])
-def test_lengths_outside_the_cache_count_as_the_nearest_inside(T):
+@pytest.mark.parametrize("T,cap", [(1, 90), (40, 90), (40, 1100)])
+def test_lengths_outside_the_cache_count_as_the_nearest_inside(T, cap):
     rng = np.random.default_rng(6)
-    H, kvh, hd, cap = 4, 2, 64, 90
+    H, kvh, hd = 4, 2, 64
     cache = Cache(rng, 3, cap, kvh, hd)
     q = rng.standard_normal((3 * T, H * hd)).astype(np.float32)
     a = run_attend(cache, q, H, T, [-5, cap - T + 1, 2 ** 31 - 1], None, None, 0)
@@ -374,7 +384,7 @@ def test_a_chain_agrees_with_the_single_token_attention():
 @pytest.mark.parametrize("some", [False, True])
 def test_accumulated_weights(lens, T, H, kvh, hd, kind, window, ring, some):
     rng = np.random.default_rng(sum(lens) * 3 + T * 5 + H + hd + some)
-    cache, q, mask, pos = setup(rng, lens, T, H, kvh, hd, kind, window, ring)
+    cache, q, mask, pos = setup(rng, lens, T, H, kvh, hd, kind, window, ring, ROOM[some])
     (kv, qd, ld, w, pd, _, lse), weights, S = check_attend(cache, q, H, T, lens, mask, pos, window)
     take = rng.integers(0, 2, (len(lens), T)).astype(np.uint8) if some else None
     want = accum64(cache, weights, T, lens, take, np.float32(0.9), None)
@@ -412,12 +422,12 @@ def test_decode_step_with_accumulation(lens, H, kvh, hd):
 
 
 @gpu
-@pytest.mark.parametrize("T", [3, 50])
-def test_lse_by_head(T):
+@pytest.mark.parametrize("T,room", [(3, 5), (50, 5), (50, 1200)])
+def test_lse_by_head(T, room):
     """lse as [heads][nodes]: the same values, written and read through its strides."""
     rng = np.random.default_rng(T)
     lens, H, kvh, hd = [140], 8, 2, 64
-    cache, q, mask, pos = setup(rng, lens, T, H, kvh, hd)
+    cache, q, mask, pos = setup(rng, lens, T, H, kvh, hd, extra=room)
     kv, qd, ld, w, pd, out, lse = run_attend(cache, q, H, T, lens, mask, pos, 0)
     by_head = torch.zeros(H, T, device="cuda").t()
     D.attend_tree_q8(out.clone(), qd, kv, H, T, ld, mask=w, pos=pd, lse=by_head)

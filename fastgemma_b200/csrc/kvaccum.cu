@@ -201,7 +201,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       float old = 0.0f;
       if (quarter == 0 && pos >= 0 && pos < len) old = p.decay * acc[x];
       float sum = 0.0f;
-      auto block = [&](int blk, auto is_masked) {
+      // seen: the block's rows that see the slot, where not all of them do
+      auto block = [&](uint32_t seen, auto is_masked) {
         constexpr bool masked = decltype(is_masked)::value;
         const int buf = u % kBufs, c0 = quarter * kQuarter;
         uint32_t s[kQuarter];
@@ -209,17 +210,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float *ca = &s_cst[buf][0][c0], *cz = &s_cst[buf][1][c0];
         const uint64_t k2 = pair2(scale, scale), l2 = pair2(kLog2e, kLog2e);
         uint64_t add = 0;
-        // which of these rows see the slot: each node's bit, once per head
-        uint32_t seen = 0;
-        if (masked) {
-          int n = (blk * kTM + c0) / G, g = blk * kTM + c0 - n * G;
-          const int w = n >> 6, sh = n & 63;
-          uint64_t by = s_by[in_tile][w] >> sh;
-          if (w < 3 && sh) by |= s_by[in_tile][w + 1] << (64 - sh);
-          const uint32_t heads = G >= 32 ? ~0u : (1u << G) - 1;
-          for (int c = -g; c < kQuarter; c += G, by >>= 1)
-            if (by & 1) seen |= c < 0 ? heads >> -c : heads << c;
-        }
         tc::tmem_wait_ld();
 #pragma unroll
         for (int c = 0; c < kQuarter; c += 4) {
@@ -277,9 +267,27 @@ __global__ void __launch_bounds__(kThreads, 1)
             wait(&bar.c_full[buf], (u / kBufs) & 1);
             wait(&bar.d_full[buf], (u / kBufs) & 1);
             tc::fence_after_sync();
-            if (blk * kTM + quarter * kQuarter < R) {
-              if (masked) block(blk, std::true_type());
-              else block(blk, std::false_type());
+            const int row = blk * kTM + quarter * kQuarter;  // the thread's first
+            if (row < R && !masked) {
+              block(~0u, std::false_type());
+            } else if (row < R) {
+              // bits of these rows' nodes: often none, or all, of a warp's slots are seen
+              const int n = quick_div(row, G), last = quick_div(min(row + kQuarter, R) - 1, G);
+              const int w = n >> 6, sh = n & 63;
+              uint64_t by = s_by[in_tile][w] >> sh;
+              if (w < 3 && sh) by |= s_by[in_tile][w + 1] << (64 - sh);
+              const uint64_t nodes = (2ull << (last - n)) - 1;
+              by &= nodes;
+              if (__all_sync(0xffffffffu, by == nodes)) {
+                block(~0u, std::false_type());
+              } else if (__any_sync(0xffffffffu, by != 0)) {
+                // each node's bit once per head
+                const uint32_t heads = (1u << G) - 1;
+                uint32_t seen = 0, bits = (uint32_t)by;
+                for (int c = n * G - row; c < kQuarter; c += G, bits >>= 1)
+                  if (bits & 1) seen |= c < 0 ? heads >> -c : heads << c;
+                block(seen, std::true_type());
+              }
             }
             tc::fence_before_sync();
             tc::mbar_arrive(&bar.d_empty[buf]);

@@ -182,15 +182,16 @@ __device__ __forceinline__ uint32_t rank_key(float v) {
 }
 
 // A cluster of CTAs per sequence, a run of slots each.  The budget-th largest
-// key comes from four passes of 256 counters over its bytes, summed over the
-// cluster through distributed shared memory; then every warp walks its share
-// of the run, 32 slots at a time, and leaves the kept ones as a bitmask with
-// the number kept before each word.  Kept slots past the budget write
-// themselves, by rank, into a list spread over the cluster (where the keys
-// were); the evicted slots below it read their source there.  Bound by
-// latency: eight cluster barriers and a pass or two over the slots for each,
-// which is why a run is short (kRunSlots) and its keys stay in shared memory
-// (CACHED; longer runs read acc and tpos again in every pass).
+// key comes from passes of 256 counters over its bytes, summed over the cluster
+// through distributed shared memory, until the keys that share the bytes so far
+// all stay (`exact`) or the four bytes are known; then every warp walks its
+// share of the run, 32 slots at a time, and leaves the kept ones as a bitmask
+// with the number kept before each word.  Each CTA lists its kept slots past
+// the budget (where the keys were); the evicted slots below it find their
+// sources there, by rank over the lists.  Bound by latency: a cluster barrier
+// and a pass or two over the slots for each of six to nine steps, which is why
+// a run is short (kRunSlots) and its keys stay in shared memory (CACHED; longer
+// runs read acc and tpos again in every pass).
 constexpr int kRunSlots = 2048, kCachedKeys = 40960;
 
 constexpr int kMaxCluster = 8;
@@ -201,7 +202,7 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictPar
   __shared__ unsigned hist[4][256], total[256];
   __shared__ int s_warp[kPlanThreads / 32], s_newest, s_eq, s_kept, s_kept_low;
   __shared__ uint32_t s_prefix;
-  __shared__ int s_left;
+  __shared__ int s_left, s_exact;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = CLUSTER ? (int)cluster.num_blocks() : 1;
   const int rank = CLUSTER ? (int)cluster.block_rank() : 0;
@@ -231,31 +232,33 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictPar
     return;
   }
   const int words = ((n + C - 1) / C + 31) / 32, run = words * 32;  // of one CTA
-  // list entries of one CTA: at most half of the slots are kept past the budget
-  // (each fills an evicted one below it)
-  const int part = run / 2;
   const int first = min(n, rank * run), last = min(n, first + run);
   const int per_warp = (words + kPlanThreads / 32 - 1) / (kPlanThreads / 32);
   uint32_t *bits = smem, *before = smem + words, *keys = before + words;
+  // kept slots past the budget, from the run's first; a run has at most 65536
+  uint16_t *list = reinterpret_cast<uint16_t *>(keys);
   // a word of every CTA of the cluster, all asked for at once (0 past the last)
   auto all = [&](int *w, int (&v)[kMaxCluster]) {
 #pragma unroll
     for (int r = 0; r < kMaxCluster; r++)
       v[r] = !CLUSTER ? (r == 0 ? *w : 0) : r < C ? *cluster.map_shared_rank(w, r) : 0;
   };
-  auto entry = [&](int i) {  // of the list
-    return CLUSTER ? cluster.map_shared_rank(keys, i / part) + i % part : keys + i;
-  };
 
   // the newest position (the slot's index where no positions are kept)
-  if (tid == 0) s_newest = INT_MIN;
+  if (tid == 0) {
+    s_newest = INT_MIN;
+    s_kept_low = 0;
+  }
   for (int i = tid; i < 4 * 256; i += kPlanThreads) (&hist[0][0])[i] = 0;
   __syncthreads();
   int newest = n - 1;
   if (tp) {
     newest = INT_MIN;
 #pragma unroll 4
-    for (int x = first + tid; x < last; x += kPlanThreads) newest = max(newest, tp[x]);
+    for (int x = first + tid; x < last; x += kPlanThreads) {
+      if (CACHED) keys[x - first] = rank_key(acc[x]);
+      newest = max(newest, tp[x]);
+    }
     newest = __reduce_max_sync(0xffffffffu, newest);
     if (lane == 0) atomicMax(&s_newest, newest);
     sync();
@@ -269,13 +272,15 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictPar
   const long long old = (long long)newest - p.recent;
   auto make_key = [&](int x) -> uint32_t {
     const int t = tp ? tp[x] : x;
-    return t < p.sink || t > old ? 0xFFFFFFFFu : rank_key(acc[x]);
+    if (t < p.sink || t > old) return 0xFFFFFFFFu;
+    return CACHED && tp ? keys[x - first] : rank_key(acc[x]);
   };
   auto key = [&](int x) -> uint32_t { return CACHED ? keys[x - first] : make_key(x); };
 
   uint32_t prefix = 0;
-  int left = budget;  // keys still to take among those that share the prefix
-  for (int pass = 0; pass < 4; pass++) {
+  int left = budget;   // keys still to take among those that share the prefix
+  bool exact = false;  // all of them are
+  for (int pass = 0; pass < 4 && !exact; pass++) {
     const int shift = 24 - 8 * pass;
 #pragma unroll 4
     for (int x = first + tid; x < last; x += kPlanThreads) {
@@ -312,6 +317,7 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictPar
           if (taken + c[i] >= left) {
             s_prefix = prefix | ((uint32_t)(255 - 8 * lane - i) << shift);
             s_left = left - taken;
+            s_exact = taken + c[i] == left;
             break;
           }
           taken += c[i];
@@ -321,6 +327,7 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictPar
     __syncthreads();
     prefix = s_prefix;
     left = s_left;
+    exact = s_exact;
   }
 
   // keys above the threshold stay, and of the equal ones the first `left`
@@ -343,29 +350,31 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictPar
     }
     return sum;  // of thread 0
   };
-  int count = 0;
-  for (int w = w0; w < w1; w++) {
-    const int x = first + w * 32 + lane;
-    count += __popc(__ballot_sync(0xffffffffu, x < last && key(x) == prefix));
-  }
-  int sum = scan_warps(count);
-  if (tid == 0) s_eq = sum;
-  sync();
-  int seen = s_warp[warp];  // equal keys before this warp's
   int v[kMaxCluster], lows[kMaxCluster];
-  all(&s_eq, v);
+  int seen = 0;  // equal keys before this warp's
+  if (!exact) {
+    int count = 0;
+    for (int w = w0; w < w1; w++) {
+      const int x = first + w * 32 + lane;
+      count += __popc(__ballot_sync(0xffffffffu, x < last && key(x) == prefix));
+    }
+    const int sum = scan_warps(count);
+    if (tid == 0) s_eq = sum;
+    sync();
+    seen = s_warp[warp];
+    all(&s_eq, v);
 #pragma unroll
-  for (int r = 0; r < kMaxCluster; r++)
-    if (r < rank) seen += v[r];
-  __syncthreads();
-  count = 0;
-  int count_low = 0;
+    for (int r = 0; r < kMaxCluster; r++)
+      if (r < rank) seen += v[r];
+    __syncthreads();
+  }
+  int count = 0, count_low = 0;
   for (int w = w0; w < w1; w++) {
     const int x = first + w * 32 + lane;
     const uint32_t k = x < last ? key(x) : 0;
     const unsigned eq = __ballot_sync(0xffffffffu, x < last && k == prefix);
-    const bool keep =
-        x < last && (k > prefix || (k == prefix && seen + __popc(eq & ((1u << lane) - 1)) < left));
+    const bool tie = k == prefix && seen + __popc(eq & ((1u << lane) - 1)) < left;
+    const bool keep = x < last && (exact ? k >= prefix : k > prefix || tie);
     const unsigned kept = __ballot_sync(0xffffffffu, keep);
     count_low += __popc(__ballot_sync(0xffffffffu, keep && x < budget));
     seen += __popc(eq);
@@ -375,39 +384,41 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictPar
     }
     count += __popc(kept);
   }
-  if (tid == 0) s_kept_low = 0;
-  sum = scan_warps(count);  // its barrier comes before the sums below
-  if (tid == 0) s_kept = sum;
   if (lane == 0 && count_low) atomicAdd(&s_kept_low, count_low);
+  const int sum = scan_warps(count);
+  if (tid == 0) s_kept = sum;
+  __syncthreads();
+  // kept slots past the budget into the CTA's list, which takes the keys' place
+  const int mine = s_warp[warp], low = s_kept_low;
+  for (int w = w0; w < w1; w++) {
+    const uint32_t word = bits[w];
+    const int at = mine + (int)before[w] + __popc(word & ((1u << lane) - 1));
+    __syncwarp();
+    if (lane == 0) before[w] = mine + (int)before[w];
+    if (first + w * 32 + lane >= budget && ((word >> lane) & 1))
+      list[at - low] = (uint16_t)(w * 32 + lane);
+  }
   sync();
-  int base = s_warp[warp], low = 0;  // kept before this warp's slots; kept below the budget
+  // kept slots of the runs before this one; entries of every list
+  int base = 0;
   all(&s_kept, v);
   all(&s_kept_low, lows);
 #pragma unroll
-  for (int r = 0; r < kMaxCluster; r++) {
+  for (int r = 0; r < kMaxCluster; r++)
     if (r < rank) base += v[r];
-    low += lows[r];
-  }
-  // kept slots past the budget into the list, which takes the keys' place
-  for (int w = w0; w < w1; w++) {
-    const int x = first + w * 32 + lane;
-    const uint32_t word = bits[w];
-    const int at = base + (int)before[w] + __popc(word & ((1u << lane) - 1));
-    __syncwarp();
-    if (lane == 0) before[w] = base + (int)before[w];
-    if (x >= budget && ((word >> lane) & 1)) {
-      const int i = at - low;
-      *entry(i) = (uint32_t)x;
-    }
-  }
-  sync();
   for (int x = first + tid; x < min(last, budget); x += kPlanThreads) {
     const int w = (x - first) >> 5;
     const uint32_t word = bits[w], bit = 1u << (x & 31);
     int s = x;
     if (!(word & bit)) {  // as many evicted slots lie before it as kept ones before its source
-      const int i = x - ((int)before[w] + __popc(word & (bit - 1)));
-      s = (int)*entry(i);
+      int i = x - (base + (int)before[w] + __popc(word & (bit - 1))), from = 0;
+#pragma unroll
+      for (int r = 0; r < kMaxCluster - 1; r++)
+        if (from == r && i >= v[r] - lows[r]) {
+          i -= v[r] - lows[r];
+          from++;
+        }
+      s = from * run + (CLUSTER ? *cluster.map_shared_rank(list + i, from) : list[i]);
     }
     map[x] = s;
     place(x, s);

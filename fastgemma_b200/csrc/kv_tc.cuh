@@ -15,6 +15,19 @@ constexpr int kTM = 128;          // query rows per tile
 constexpr int kTN = 128;          // slots per tile
 constexpr int kChunk = 128 * 128; // bytes of one 128-byte column of Q or of a K tile
 
+// Whether this is the warp's elected lane.  The warp that issues the MMAs runs
+// as a whole, so that descriptors and counters stay in uniform registers, and
+// elects a lane for the instructions of one thread.
+__device__ __forceinline__ bool elected() {
+  uint32_t is;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(is));
+  return is != 0;
+}
+
 __device__ __forceinline__ uint64_t desc128(uint32_t a) { return tc::sdesc_sw128(a); }
 
 // D[tmem] (+)= A[tmem, f16] * B[smem desc, f16], f32 accumulate.
@@ -136,8 +149,8 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 
 // Waits until the phase with `parity` is over.  The tests put the warp to sleep
 // for up to 10 us each: spinning, or reading a clock or the abort word between
-// the tests, takes issue slots from the warps that work (chunk_256_16k 61.7 us
-// like this, 65 to 71 otherwise).  After kWaitTests tests, two seconds asleep,
+// the tests, takes issue slots from the warps that work (256 nodes over 16K
+// slots 65.7 us like this, 68.9 when the MMA warp alone spins, 71 when all do).  After kWaitTests tests, two seconds asleep,
 // the wait gives up and raises the abort word, on which later waits do not
 // sleep any more: the loops run out, the CTA reports and leaves.
 constexpr int kWaitTests = 200000;

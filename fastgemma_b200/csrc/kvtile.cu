@@ -8,21 +8,31 @@
 // and write the weights p * vs to TMEM as two f16 parts (22 bits together, as
 // in the streaming kernel), 64 slots a buffer; those are the A operand of two
 // products with V (kind::f16) that add into the f32 output in TMEM.  So no
-// MMA is waited for before the next is issued, only their inputs are.  V comes from the cache
-// as int8, four slots of a dimension per word; four warps load it and write
-// the f16 B operand (exact), 64 slots at a time.  The output is rescaled only
-// when a row's maximum has grown by more than 2^8: until then the weights just
-// grow, for which the f16 scale leaves room.
+// MMA is waited for before the next is issued, only their inputs are.  V comes
+// from the cache as int8, four slots of a dimension per word; four warps load
+// it and write the f16 B operand (exact), 64 slots at a time.  The output is
+// rescaled only when a row's maximum has grown by more than 2^8: until then the
+// weights just grow, for which the f16 scale leaves room.
 //
 // The queries are quantised once, by a kernel before, into the swizzled blocks
-// that the tiles copy (each CTA for itself took 6 us more at chunk_256_16k: nine
-// CTAs then read the same 128 KB); partial results of items split over CTAs
-// are joined by a kernel after.
+// that the tiles copy (each CTA for itself took 6 us more at 256 nodes over 16K
+// slots: nine CTAs then read the same 128 KB); partial results of items split
+// over CTAs are joined by a kernel after.
 //
-// Bound by the tensor cores: a tile costs 128 * 128 * hd MACs at the int8 rate
-// and twice that at the f16 rate.  Shared memory is next: both operands of the
-// scores and V (twice) come from it, which is why V passes through registers
-// instead of being staged as int8.
+// A tile costs 128 * 128 * hd MACs at the int8 rate and twice that at the f16
+// rate, 1.45 us at head_dim 256, and takes 3.0: the MMAs, in the order of their
+// issue, the softmax (2.5 us) and the conversion (2.6 us, half of it waiting
+// for loads and stores to land) each wait for the others once per tile.  Left
+// out one at a time they gain 3 us (conversion) and 7 us (softmax) of 65, both
+// together 18.  Beside the tiles a call costs 23 us: the quantisation 4, setup
+// 3 (under it), the way to the first weights 4, the last product and 128 KB of
+// partial results a CTA 5, the join 4, the rest launches.  256 nodes, 8 heads
+// over 2, head_dim 256: 65.2 us over 16K slots, 191 over 64K (720 TFLOP/s of
+// the two products; each counted once).
+//
+// Accuracy: the tensor cores add into the f32 output without rounding to
+// nearest, sixteen times per tile; over fifteen tiles that is 2.9e-6 of the
+// output's norm, where rounding every f32 step leaves 1.7e-6.
 #include <type_traits>
 
 #include "kv_tc.cuh"
@@ -185,19 +195,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::mbar_arrive(&bar.sc_full[j & 1]);
     }
   } else if (warp == 1) {  // ---- MMAs
-    if (lane == 0) {
-      // descriptors differ from these in their address field, 16 bytes a unit
-      const uint64_t qd = desc128(tc::smem_u32(q8)), kd = desc128(tc::smem_u32(ksm));
-      const uint64_t vd = desc128(tc::smem_u32(vf));
-      const uint32_t id_s = tc::idesc_i8(kTM, kTN), id_o = idesc_f16(kTM, dv);
-      int kst = 0, vst = 0;
-      uint32_t kph = 0, vph = 0;
-      auto scores = [&] {
-        const uint32_t d = tmem + kColS;
-        for (int kb = 0; kb < tp.nkb; kb++) {
-          wait(&bar.k_full[kst], kph);
-          tc::fence_after_sync();
-          const uint64_t a = qd + kb * (kChunk >> 4), c = kd + kst * (kChunk >> 4);
+    // descriptors differ from these in their address field, 16 bytes a unit
+    const uint64_t qd = desc128(tc::smem_u32(q8)), kd = desc128(tc::smem_u32(ksm));
+    const uint64_t vd = desc128(tc::smem_u32(vf));
+    const uint32_t id_s = tc::idesc_i8(kTM, kTN), id_o = idesc_f16(kTM, dv);
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const int n = __shfl_sync(0xffffffffu, tiles, 0);
+    int kst = 0, vst = 0;
+    uint32_t kph = 0, vph = 0;
+    auto scores = [&] {
+      const uint32_t d = tm + kColS;
+      for (int kb = 0; kb < tp.nkb; kb++) {
+        wait(&bar.k_full[kst], kph);
+        tc::fence_after_sync();
+        const uint64_t a = qd + kb * (kChunk >> 4), c = kd + kst * (kChunk >> 4);
+        if (elected()) {
           tc::mma_i8(d, a, c, id_s, kb > 0);
           tc::mma_i8(d, a + 2, c + 2, id_s, 1);
           if (hd - kb * 128 >= 128) {
@@ -205,33 +217,37 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc::mma_i8(d, a + 6, c + 6, id_s, 1);
           }
           tc::mma_commit(&bar.k_empty[kst]);
-          if (++kst == tp.kstages) kst = 0, kph ^= 1;
+          if (kb == tp.nkb - 1) tc::mma_commit(&bar.s_full);
         }
-        tc::mma_commit(&bar.s_full);
-      };
-      wait(&bar.q_full, 0);
-      scores();
-      for (int j = 0; j < tiles; j++) {
-        if (j + 1 < tiles) {  // the next scores once these are in registers
-          wait(&bar.s_empty, j & 1);
-          scores();
-        }
+        __syncwarp();
+        if (++kst == tp.kstages) kst = 0, kph ^= 1;
+      }
+    };
+    wait(&bar.q_full, 0);
+    scores();
+    for (int j = 0; j < n; j++) {
+      if (j + 1 < n) {  // the next scores once these are in registers
+        wait(&bar.s_empty, j & 1);
+        scores();
+      }
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          wait(&bar.p_full[h], j & 1);
-          wait(&bar.v_full[vst], vph);
-          tc::fence_after_sync();
-          const uint64_t v = vd + vst * (dv * 8);
-          const uint32_t a = tmem + kColP + h * 64;
+      for (int h = 0; h < 2; h++) {
+        wait(&bar.p_full[h], j & 1);
+        wait(&bar.v_full[vst], vph);
+        tc::fence_after_sync();
+        const uint64_t v = vd + vst * (dv * 8);
+        const uint32_t a = tm + kColP + h * 64;
+        if (elected()) {
 #pragma unroll
           for (int k = 0; k < 4; k++) {
-            mma_f16_ts(tmem, a + k * 8, v + k * 2, id_o, j + h + k > 0);
-            mma_f16_ts(tmem, a + 32 + k * 8, v + k * 2, id_o, 1);
+            mma_f16_ts(tm, a + k * 8, v + k * 2, id_o, j + h + k > 0);
+            mma_f16_ts(tm, a + 32 + k * 8, v + k * 2, id_o, 1);
           }
           tc::mma_commit(&bar.v_empty[vst]);
           tc::mma_commit(&bar.p_empty[h]);
-          if (++vst == kVStages) vst = 0, vph ^= 1;
         }
+        __syncwarp();
+        if (++vst == kVStages) vst = 0, vph ^= 1;
       }
     }
   } else if (warp >= 4 + kSoftWarps) {  // ---- V to f16, K-major: a row per dimension, 64 slots
@@ -290,7 +306,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp >= 4) {  // ---- softmax: row (warp % 4) * 32 + lane, slots 32 * quarter ...
     const int quarter = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t quad = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const int r = row0 + row, node = row < rows ? r / G : -1, low = s_low[row];
     const bool idle = (warp & 3) * 32 >= rows;  // only padding rows: nothing to compute
     stream::pdl_wait();
     const float qs = row < rows ? tp.qs[qblock * kTM + row] : 1e-37f;
@@ -298,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         0xffffffffu, max(max(s_low[lane], s_low[lane + 32]), max(s_low[lane + 64], s_low[lane + 96])));
     {  // the nodes this row sees, a word per quarter
       uint64_t v = 0;
-      const int w = quarter;
+      const int w = quarter, low = s_low[row], node = row < rows ? (row0 + row) / G : -1;
       if (node >= 0 && w * 64 < p.T) {
         v = p.mask ? p.mask[((size_t)b * p.T + node) * ((p.T + 63) / 64) + w]
                    : bit_range(0, node + 1 - w * 64);
@@ -312,9 +327,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     // the four warps that share the quadrant's rows
     auto meet = [&] { asm volatile("bar.sync %0, 128;" ::"r"(1 + (warp & 3)) : "memory"); };
     meet();
-    // position of slot x: x + (x <= turn ? lo_off : hi_off)
-    const int turn = ring ? (end - 1) % ring : INT_MAX;
-    const int lo_off = ring ? end - 1 - turn : 0, hi_off = lo_off - ring;
     float m = -INFINITY, l = 0.0f;
 
     auto tile = [&](int j, auto is_masked) {
@@ -325,6 +337,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::tmem_ld_x32(quad + kColS + quarter * kQuarter, s);
       uint32_t seen = 0;
       if (masked) {
+        // position of slot x: x + (x <= turn ? lo_off : hi_off)
+        const int turn = ring ? (end - 1) % ring : INT_MAX, low = s_low[row];
+        const int lo_off = ring ? end - 1 - turn : 0, hi_off = lo_off - ring;
         const int x = x0 + j * kTN + quarter * kQuarter, cut = turn - x;
         seen = seen_from(x + (cut >= 0 ? lo_off : hi_off), len, low, s_see[row]);
         if (cut >= 0 && cut < kQuarter - 1) {  // the ring turns inside these slots
@@ -332,7 +347,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           seen = (seen & before) | (seen_from(x + hi_off, len, low, s_see[row]) & ~before);
         }
         seen &= (uint32_t)bit_range(0, x1 - x);
-        if (node < 0) seen = 0;
       }
       tc::tmem_wait_ld();
       tc::fence_before_sync();
@@ -480,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     stream::fence_proxy_async_smem();
     meet();
     if (quarter == 0 && row < rows) {
-      const int h = kvh * G + r - node * G;
+      const int r = row0 + row, node = r / G, h = kvh * G + r - node * G;
       const size_t qr = (size_t)b * p.T + node;
       bulk_s2g(whole ? p.out + qr * p.out_ld + (size_t)h * hd + ds * dv
                      : tp.part + ((size_t)blockIdx.x * kTM + row) * dv, stage, (uint32_t)dv * 4);

@@ -7,8 +7,15 @@
 // own slot's weights in a register, block after block, KV head after KV head,
 // in a fixed order and without a reduction across threads until the four
 // warps that share a lane quadrant put their quarters together.  Four score
-// buffers keep the tensor cores ahead of the exponentials, which bound it: one
-// per (query row, slot) pair at 16 a cycle per SM.
+// buffers keep the tensor cores ahead of the exponentials: one per (query row,
+// slot) pair at 16 a cycle per SM.
+//
+// 256 nodes, 8 heads over 2, over 16K slots of head_dim 256: 25.8 us, 34 M
+// exponentials (the exponential unit 42 % busy, 8.2 us alone; without any
+// arithmetic on the scores 20.6, without masks 22.8).  A launch is one tile of
+// slots per CTA, so what is left is the start of each: the quantisation before
+// it 4 us, K and the first queries 3, and 32 KB of queries per block and KV head
+// from L2.  16 nodes of 8 sequences over 4K slots: 11.9 us, latency alone.
 #include <type_traits>
 
 #include "kv_tc.cuh"
@@ -322,7 +329,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // A warp per query row of a block of 128: its int8 copy in the block's
-// swizzled place and its scale.  For the attention the scale times log2(e);
+// swizzled place and its scale; 4 us for any size in use, of which the kernel
+// after it, launched early, spends 3 on its own setup.  For the attention the scale times log2(e);
 // for the accumulation (p.decay in use, cst set) the scale itself and -lse,
 // -infinity where a row adds nothing.
 constexpr int kQuantRows = 8;

@@ -41,7 +41,8 @@ __global__ void __launch_bounds__(kTreeMax) tree_mask_kernel(uint64_t *mask, int
 }
 
 // One warp per tree: each step looks at all nodes at once for the lowest
-// right child of the last accepted one.
+// right child of the last accepted one, so the path's length, not the tree's
+// size, is what it takes.
 __global__ void __launch_bounds__(32) tree_verify_kernel(int32_t *path, int32_t *n_acc,
                                                          int32_t *next, const int32_t *parent,
                                                          const int32_t *token,
@@ -84,7 +85,9 @@ struct AcceptParams {
   int32_t *lens_new;
 };
 
-// One CTA per (sequence, layer).  Warp 0 moves K rows, 16 bytes a lane, the
+// One CTA per (sequence, layer); bound by the latency of lens, path, rows (3.7
+// us with the verification for one sequence and 4 layers, 6.6 for 8 sequences of
+// 61 nodes and 30 layers).  Warp 0 moves K rows, 16 bytes a lane, the
 // others V, a dimension's word a lane, eight path entries at a time: their
 // loads all go out before the first store.  That keeps the order right too:
 // the destination of entry j lies at or before its source and the sources
@@ -191,7 +194,9 @@ __device__ __forceinline__ uint32_t rank_key(float v) {
 // sources there, by rank over the lists.  Bound by latency: a cluster barrier
 // and a pass or two over the slots for each of six to nine steps, which is why
 // a run is short (kRunSlots) and its keys stay in shared memory (CACHED; longer
-// runs read acc and tpos again in every pass).
+// runs read acc and tpos again in every pass).  8 sequences of 16K slots: 15.8
+// us (with one CTA a sequence about 20 more), of which 2.3 until the keys are there, 1.5
+// for each barrier with its counters, 3.2 for the map; 600 slots: 6.
 constexpr int kRunSlots = 2048, kCachedKeys = 40960;
 
 constexpr int kMaxCluster = 8;
@@ -429,7 +434,11 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictPar
 
 // A warp per kMoveSlots slots of a sequence: the rows that move, their loads
 // all on the way before the first store.  Rows move from past the budget to
-// below it, so no order matters.
+// below it, so no order matters.  Bound by memory latency and by sectors that
+// are read and written for one byte in four of V: 14336 rows of 512 dimensions
+// in 16 us.  Rows listed per CTA of 64 slots before they move took 18.7, whole
+// words of V, merged and stored, 19.7, the rows past the budget asked for in L2
+// during the plan 16.6.
 constexpr int kMoveSlots = 8, kMoveWarps = 8;
 __global__ void __launch_bounds__(kMoveWarps * 32) evict_move_kernel(const EvictParams p,
                                                                      int groups) {

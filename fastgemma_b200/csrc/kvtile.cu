@@ -48,7 +48,7 @@ constexpr int kSoftWarps = 16, kSoft = kSoftWarps * 32;
 constexpr int kThreads = 128 + kSoft + 128;  // loads and MMAs, softmax, V conversion
 constexpr int kQuarter = kTN / 4;  // slots of a softmax thread
 constexpr int kGrow = 8;          // log2 by which a row's maximum may grow unnoticed
-constexpr int kUnit = 5;          // f16 weights: p * vs * 2^(kUnit - ve), at most 2^(kUnit + kGrow)
+constexpr int kUnit = 7;          // f16 weights: p * vs * 2^(kUnit - ve), below 2^(kUnit + kGrow)
 // TMEM columns: output [0, 256), scores 128, weights of 64 slots 2 x (32 high, 32 low parts)
 constexpr uint32_t kColS = 256, kColP = 384;
 
@@ -466,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     wait(&bar.p_empty[1], (tiles - 1) & 1);
     tc::fence_after_sync();
     const bool whole = wk.count == 1;
-    float back = pow2(ve) * 0.03125f;  // 2^-kUnit
+    float back = pow2(ve) * 0.0078125f;  // 2^-kUnit
     if (whole) back = L == 0.0f ? 0.0f : back / L;
     float *stage = reinterpret_cast<float *>(sm + (size_t)row * (dv * 4 + 16));
     // column e * dv / 4 + i of the output is dimension 4 i + e

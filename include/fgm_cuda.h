@@ -484,10 +484,13 @@ size_t fgm_cuda_attend_workspace(const fgm_cuda_kv *kv, int n_heads, int T);
  * Per head: q8 = rint(q * (127 / max|q|)), score = (q8 . k8) * (max|q| / 127)
  * * ks[slot] as in fgm_cuda_attend_q8; out = sum(softmax(score) * vs * v8)
  * with the weights in f32 (attend_q8 rounds them to 16 bits, as the
- * reference does, so the two differ by that).  A node that sees nothing gets
- * zeros.  lse (may be NULL): log of the sum of exp(score) of row r = b*T + i,
- * head h at lse[r * lse_row + h * lse_head]; -inf for such a node.  A query head with a value that is no
- * finite number gives not-a-number in out and lse, in that head alone.
+ * reference does, so the two differ by that), scaled by the largest |vs| that
+ * one thread block meets: a slot whose |vs| is 2^13 times below that one's
+ * weighs with 17 bits or more, still smaller ones with fewer.  A node that
+ * sees nothing gets zeros.  lse (may be NULL): log of the sum of exp(score) of
+ * row r = b*T + i, head h at lse[r * lse_row + h * lse_head]; -inf for such a
+ * node.  A query head with a value that is no finite number gives
+ * not-a-number in out and lse, in that head alone.
  * 1 <= T <= FGM_CUDA_TREE_MAX, at most 16 query heads per KV head; ring > 0
  * needs 0 < window and window + T - 1 <= ring; q, out 16-byte aligned, q_ld
  * and out_ld multiples of 4. */

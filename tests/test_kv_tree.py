@@ -286,6 +286,24 @@ def test_attend_scales_of_every_size(T, room):
 
 
 @gpu
+@pytest.mark.parametrize("T,H,kvh,hd,room", [(3, 8, 2, 256, 5), (20, 8, 2, 128, 1200),
+                                             (60, 8, 2, 256, 600)])
+def test_one_v_scale_far_above_the_others(T, H, kvh, hd, room):
+    """A slot of zeros whose scale is 2^13 times the smallest other: the others
+    keep 17 bits of their weights, so half a unit of the 17th is the error that
+    joins an output's."""
+    rng = np.random.default_rng(T)
+    lens = [300, 77]
+    cache, q, mask, pos = setup(rng, lens, T, H, kvh, hd, extra=room)
+    cache.vs[:, 7] = 0.001 * 2.0 ** 13
+    cache.v[:, 7] = 0
+    got = run_attend(cache, q, H, T, lens, mask, pos, 0)
+    want, _, _, S, V = attend64(cache, q, H, T, lens, mask, pos, 0)
+    tol = (16 * S + 64 + (max(lens) + T) / 8) * EPS + 2.0 ** -18
+    assert np.abs(got[5].cpu().numpy() - want).max() <= tol * V
+
+
+@gpu
 @pytest.mark.parametrize("T,hd,room", [(2, 128, 5), (48, 256, 5), (48, 256, 300), (48, 64, 1200)])
 def test_a_query_that_is_no_number_stays_in_its_head(T, hd, room):
     rng = np.random.default_rng(5)

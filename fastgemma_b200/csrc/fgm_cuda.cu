@@ -1759,6 +1759,7 @@ int fgm_cuda_tree_mask(uint64_t *mask, int32_t *pos, const int32_t *parent, cons
                 FGM_CUDA_TREE_MAX);
   if (rows == 0) return FGM_CUDA_OK;
   if (!mask || !parent || (pos && !lens)) return fail(FGM_CUDA_EINVAL, "tree_mask: null pointer");
+  if (addr(mask) & 7) return fail(FGM_CUDA_EINVAL, "tree_mask: mask must be 8-byte aligned");
   return glue_done(launch_tree_mask(mask, pos, parent, lens, rows, T, (cudaStream_t)stream),
                    "tree_mask launch");
 }
@@ -1779,7 +1780,10 @@ int fgm_cuda_attend_tree_q8(const fgm_cuda_kv *kv, const float *q, int q_ld, int
   if ((rc = check_attend("attend_tree", p, ws_bytes, true)) || kv->rows == 0) return rc;
   DevInfo *di = nullptr;
   if ((rc = dev_info(&di))) return rc;
-  return glue_done(launch_attend_tree(p, di->sms, di->err, (cudaStream_t)stream), "attend_tree launch");
+  int launches = 0;
+  const cudaError_t e = launch_attend_tree(p, di->sms, di->err, &launches, (cudaStream_t)stream);
+  count_launch(launches);
+  return e == cudaSuccess ? FGM_CUDA_OK : cuda_fail(e, "attend_tree launch");
 }
 
 int fgm_cuda_attend_accum_q8(const fgm_cuda_kv *kv, const float *q, int q_ld, int n_heads, int T,
@@ -1795,8 +1799,10 @@ int fgm_cuda_attend_accum_q8(const fgm_cuda_kv *kv, const float *q, int q_ld, in
   if (!lse || !kv->acc) return fail(FGM_CUDA_EINVAL, "attend_accum: null pointer (lse, kv->acc)");
   DevInfo *di = nullptr;
   if ((rc = dev_info(&di))) return rc;
-  return glue_done(launch_attend_accum(p, di->sms, di->err, (cudaStream_t)stream),
-                   "attend_accum launch");
+  rc = glue_done(launch_attend_accum(p, di->sms, di->err, (cudaStream_t)stream),
+                 "attend_accum launch");
+  if (!rc) count_launch();
+  return rc;
 }
 
 int fgm_cuda_attend_acc_q8(const fgm_cuda_kv *kv, const float *q, int q_ld, int n_heads,

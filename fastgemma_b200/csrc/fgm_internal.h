@@ -187,7 +187,8 @@ struct TreeParams {
   void *ws;
 };
 size_t attend_workspace(const fgm_cuda_kv &kv, int n_heads, int T);
-cudaError_t launch_attend_tree(const TreeParams &p, int num_sms, int *err, cudaStream_t st);
+cudaError_t launch_attend_tree(const TreeParams &p, int num_sms, int *err, int *launches,
+                               cudaStream_t st);
 // kvtile.cu, more than 16 query rows per KV head; err: set when a wait gives up
 size_t attend_tile_workspace(const fgm_cuda_kv &kv, int n_heads, int T);
 cudaError_t launch_attend_tile(const TreeParams &p, int num_sms, int *err, cudaStream_t st);

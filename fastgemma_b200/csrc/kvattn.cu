@@ -586,9 +586,13 @@ size_t attend_workspace(const fgm_cuda_kv &kv, int n_heads, int T) {
   return std::max(n, accum_workspace(kv, n_heads, T));
 }
 
-cudaError_t launch_attend_tree(const TreeParams &p, int num_sms, int *err, cudaStream_t st) {
-  if (!streams(p)) return launch_attend_tile(p, num_sms, err, st);
-  return launch_stream(p, false, num_sms, st);
+cudaError_t launch_attend_tree(const TreeParams &p, int num_sms, int *err, int *launches,
+                               cudaStream_t st) {
+  const bool tiles = !streams(p);
+  const cudaError_t e = tiles ? launch_attend_tile(p, num_sms, err, st)
+                              : launch_stream(p, false, num_sms, st);
+  if (e == cudaSuccess) *launches = tiles ? 3 : 1;
+  return e;
 }
 
 cudaError_t launch_attend_acc(const TreeParams &p, int num_sms, cudaStream_t st) {

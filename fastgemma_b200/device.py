@@ -260,11 +260,18 @@ def kv_layers(views):
     return arr
 
 
+_NOT_INT32 = {"mask": torch.int64, "take": torch.uint8}
+
+
 def _flat(**tensors):
-    """The entries take whole tensors by address: a strided one would be misread."""
+    """The entries take whole tensors by address: one of another type, or a
+    strided one, would be misread."""
     for name, t in tensors.items():
-        if t is not None and not t.is_contiguous():
-            raise ValueError(f"{name} has to be contiguous")
+        if t is not None and (t.dtype != _NOT_INT32.get(name, torch.int32) or
+                              not t.is_contiguous()):
+            raise ValueError(f"{name} has to be contiguous "
+                             f"{_NOT_INT32.get(name, torch.int32)}, not {t.dtype} with strides "
+                             f"{t.stride()}")
 
 
 def _lse(lse):
@@ -325,6 +332,7 @@ def attend_accum_q8(q, kv, n_heads, T, lens, lse, mask=None, pos=None, window=0,
 def attend_acc_q8(out, q, kv, n_heads, lens, decay=1.0, ws=None, q_ld=None, out_ld=None,
                   stream=None):
     """One token per sequence: attention over slots [0, lens[b]] and its weights added to kv's acc."""
+    _flat(lens=lens)
     ws = _ws(ws, kv, n_heads, 1, stream)
     ld = n_heads * kv.head_dim
     call("fgm_cuda_attend_acc_q8", C.byref(kv), _p(q), ld if q_ld is None else q_ld, n_heads,
@@ -336,7 +344,7 @@ def tree_verify(path, n_acc, next_token, parent, token, target, stream=None):
     """The accepted path of each drafted tree: path [rows][T] (then -1), its
     length n_acc and the token after it."""
     rows, T = parent.shape
-    _flat(path=path, parent=parent, token=token, target=target)
+    _flat(path=path, n_acc=n_acc, next_token=next_token, parent=parent, token=token, target=target)
     call("fgm_cuda_tree_verify", _p(path), _p(n_acc), _p(next_token), _p(parent), _p(token),
          _p(target), rows, T, _s(stream))
 
@@ -344,7 +352,7 @@ def tree_verify(path, n_acc, next_token, parent, token, target, stream=None):
 def kv_accept(layers, T, lens, path, n_acc, lens_new=None, stream=None):
     """Move the accepted path's rows behind the committed ones in every layer
     (layers: kv_layers(...) or one KvCache)."""
-    _flat(lens=lens, path=path, n_acc=n_acc)
+    _flat(lens=lens, path=path, n_acc=n_acc, lens_new=lens_new)
     one = isinstance(layers, KvCache)
     call("fgm_cuda_kv_accept", C.byref(layers) if one else layers, 1 if one else len(layers), T,
          _p(lens), _p(path), _p(n_acc), _p(lens_new), _s(stream))
@@ -366,6 +374,7 @@ def kv_evict_q8(kv, lens, budget, sink, recent, slot_map, lens_out, acc_out=None
 def qkv_post_tree(kv, q, k, v, n_heads, T, q_norm, k_norm, eps, inv_freq, pos, lens, q_ld=None,
                   kv_ld=None, cs=None, stream=None):
     """qkv_post for the nodes of a tree: rope at pos, K / V rows into slots lens[b] + i."""
+    _flat(pos=pos, lens=lens)
     kvd = kv.kv_heads * kv.head_dim
     call("fgm_cuda_qkv_post_tree", C.byref(kv), _p(q),
          n_heads * kv.head_dim if q_ld is None else q_ld, _p(k), _p(v),

@@ -803,6 +803,7 @@ def test_other_refusals():
     assert verify(FAKE, FAKE, None, FAKE, FAKE, FAKE, 1, 4, None) == -1 and "null" in err()
     assert L.fgm_cuda_tree_mask(FAKE, FAKE, FAKE, None, 1, 4, None) == -1 and "null" in err()
     assert L.fgm_cuda_tree_mask(FAKE, None, FAKE, None, 1, 257, None) == -1 and "T=257" in err()
+    assert L.fgm_cuda_tree_mask(FAKE + 4, None, FAKE, None, 1, 4, None) == -1 and "8-byte" in err()
     assert L.fgm_cuda_kv_accept(p, 1, 65, FAKE, FAKE, FAKE, None, None) == -1 and "T=65" in err()
     assert L.fgm_cuda_kv_accept(p, 1, 2, FAKE, FAKE, FAKE, FAKE, None) == -1 and "lens_new" in err()
     two = (D.KvCache * 2)(view(), view(rows=1))
@@ -845,6 +846,8 @@ def test_views_check_their_tensors():
         D.KvCache(kc, s, vt, s, 1, 64, acc=torch.zeros(2, 7))
     with pytest.raises(ValueError, match="mask has to be contiguous"):
         D._flat(lens=None, mask=torch.zeros(4, 4).t())
+    with pytest.raises(ValueError, match="lens has to be contiguous torch.int32, not torch.int64"):
+        D._flat(lens=torch.tensor([3, 4]))
 
 
 # ------------------------------------------------------------- all together

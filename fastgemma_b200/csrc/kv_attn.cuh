@@ -88,8 +88,9 @@ __device__ __forceinline__ Span span_of(const TreeParams &p, int b) {
 // an item's tiles per CTA.  Lengths are known on the device only, so every
 // warp finds its CTA's run itself: the fewest tiles per CTA for which all runs
 // fit the grid, which holds at least one CTA per item; where no item has more
-// than `whole` tiles, one CTA takes each, which spares the join.  Splitting items instead of a flat list of tiles costs at most one
-// tile of balance and saves a CTA from working on two items in turn (5 us).
+// than `whole` tiles, one CTA takes each, which spares the join.  Splitting items
+// instead of a flat list of tiles costs at most one tile of balance and saves a
+// CTA from working on two items in turn (5 us).
 constexpr int kCounters = 16384;  // grid of a launch with split items, at most
 
 struct Work {
@@ -112,10 +113,11 @@ __device__ __forceinline__ int quick_div(int x, int d) {
   return r < 0 ? q - 1 : (r >= d ? q + 1 : q);
 }
 
+// seq: not a CTA's own run but a sequence's first (of the launch of `grid` CTAs).
 template <bool ALL = false>
 __device__ __forceinline__ bool find_work(const TreeParams &p, int tile, int per_b, int whole,
-                                          int lane, Work &w) {
-  const int rows = p.kv.rows, grid = gridDim.x, cta = blockIdx.x;
+                                          int lane, Work &w, int grid, int cta, int seq = -1) {
+  const int rows = p.kv.rows;
   const Span mine = span_of<ALL>(p, min(lane, rows - 1));
   const int n0 = lane < rows ? tiles_of(mine, tile) : 0;  // the first 32 sequences stay here
   int total = n0, longest = n0;
@@ -146,7 +148,7 @@ __device__ __forceinline__ bool find_work(const TreeParams &p, int tile, int per
       const int v = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += v;
     }
-    const unsigned hit = __ballot_sync(0xffffffffu, base + inc > cta);
+    const unsigned hit = __ballot_sync(0xffffffffu, seq >= 0 ? b == seq : base + inc > cta);
     if (hit) {
       const int l = __ffs(hit) - 1;
       const int t = __shfl_sync(0xffffffffu, tiles, l);
@@ -155,10 +157,11 @@ __device__ __forceinline__ bool find_work(const TreeParams &p, int tile, int per
       w.span.end = __shfl_sync(0xffffffffu, s.end, l);
       w.b = b0 + l;
       w.count = __shfl_sync(0xffffffffu, cnt, l);
-      const int rel = cta - base - __shfl_sync(0xffffffffu, inc - cnt * per_b, l);
+      const int start = base + __shfl_sync(0xffffffffu, inc - cnt * per_b, l);
+      const int rel = seq >= 0 ? 0 : cta - start;
       w.in_b = quick_div(rel, w.count);
       const int k = rel - w.in_b * w.count, each = quick_div(t, w.count), more = t - each * w.count;
-      w.first = cta - k;
+      w.first = start + rel - k;
       w.t0 = k * each + min(k, more);
       w.t1 = w.t0 + each + (k < more);
       return true;
@@ -166,6 +169,50 @@ __device__ __forceinline__ bool find_work(const TreeParams &p, int tile, int per
     base += __shfl_sync(0xffffffffu, inc, 31);
   }
   return false;
+}
+
+template <bool ALL = false>
+__device__ __forceinline__ bool find_work(const TreeParams &p, int tile, int per_b, int whole,
+                                          int lane, Work &w) {
+  return find_work<ALL>(p, tile, per_b, whole, lane, w, gridDim.x, blockIdx.x);
+}
+
+// Four dimensions of a row from its parts (their maxima and sums `stat`), the
+// first parts' values asked for together with their statistics.
+struct Joined {
+  float4 a;
+  float M, L;
+};
+__device__ __forceinline__ Joined join_row4(const float2 *stat, const float4 *part, size_t stat_ld,
+                                            size_t part_ld, int count) {
+  Joined j{make_float4(0, 0, 0, 0), -INFINITY, 0.0f};
+  constexpr int kParts = 12;
+  for (int i0 = 0; i0 < count; i0 += kParts) {
+    float2 s[kParts];
+    float4 v[kParts];
+    const int n = min(kParts, count - i0);
+#pragma unroll
+    for (int i = 0; i < kParts; i++) {
+      s[i] = i < n ? stat[(i0 + i) * stat_ld] : make_float2(-INFINITY, 0.0f);
+      v[i] = i < n ? part[(i0 + i) * part_ld] : make_float4(0, 0, 0, 0);
+    }
+    float N = j.M;
+#pragma unroll
+    for (int i = 0; i < kParts; i++) N = fmaxf(N, s[i].x);
+    const float ref = N == -INFINITY ? 0.0f : N, f0 = ex2(j.M - ref);
+    j.a.x *= f0, j.a.y *= f0, j.a.z *= f0, j.a.w *= f0;
+    j.L *= f0;
+#pragma unroll
+    for (int i = 0; i < kParts; i++) {
+      const float f = ex2(s[i].x - ref);
+      j.L += f * s[i].y;
+      j.a.x += f * v[i].x, j.a.y += f * v[i].y, j.a.z += f * v[i].z, j.a.w += f * v[i].w;
+    }
+    j.M = N;
+  }
+  const float inv = j.L == 0.0f ? 0.0f : 1.0f / j.L;
+  j.a.x *= inv, j.a.y *= inv, j.a.z *= inv, j.a.w *= inv;
+  return j;
 }
 
 // What the attention kernels leave behind for an item that several CTAs work

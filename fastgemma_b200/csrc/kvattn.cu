@@ -70,10 +70,10 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
 // split into two f16 (scaled by a running power of two above the largest
 // |vs|), 22 bits in all, so the products lose less than f32 rounding does.
 //
-// 8 sequences of up to 32K slots, 8 heads over 2 of head_dim 256: 52 us for
-// 212 MB (4.1 TB/s over the launch, 6 to 7 while the rings run; 36 % of the
+// 8 sequences of up to 32K slots, 8 heads over 2 of head_dim 256: 50 us for
+// 212 MB (4.2 TB/s over the launch, 6 to 7 while the rings run; 36 % of the
 // issue slots, 18 % of the tensor cycles): 6 us before the first stage has
-// landed, up to 6 % longer runs on some CTAs, 3 to 5 for the join.  Two CTAs an
+// landed, up to 6 % longer runs on some CTAs, 3 to 5 for a join.  Two CTAs an
 // SM with rings of half the length took 54.  Short calls are latency: 4 nodes
 // over 96 slots 9.7 us.
 constexpr int kTile = 128;   // slots per tile of the work list
@@ -99,7 +99,7 @@ struct StreamParams {
   TreeParams t;
   Parts parts;
   int blocks;       // row blocks per (sequence, KV head)
-  float *scores;    // [rows][n_heads][score_ld], or null
+  float *scores;    // [rows][n_heads][score_ld], or null: no accumulation behind
   int score_ld;
 };
 
@@ -419,6 +419,7 @@ __global__ void __launch_bounds__(stream_warps(HD) * 32, 1)
   __syncthreads();
   const float back = pow2(e_all) * 0.0001220703125f;  // 2^-13
   const int rows = min(ROWS, R - row0);
+  const bool whole = wk.count == 1 && !sp.scores;  // with scores the next kernel joins
   for (int i = tid; i < rows * (HD / 4); i += W * 32) {
     const int row = i / (HD / 4), d = (i - row * (HD / 4)) * 4;
     float4 a = make_float4(0, 0, 0, 0);
@@ -428,46 +429,94 @@ __global__ void __launch_bounds__(stream_warps(HD) * 32, 1)
       a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
     }
     a.x *= back, a.y *= back, a.z *= back, a.w *= back;
-    if (wk.count == 1) {
+    if (whole) {
       store_row4(p, wk, kvh, row0 + row, d, a, s_M[row], s_L[row]);
     } else {
       *reinterpret_cast<float4 *>(sp.parts.part + ((size_t)blockIdx.x * ROWS + row) * HD + d) = a;
       if (d == 0) sp.parts.stat[(size_t)blockIdx.x * ROWS + row] = make_float2(s_M[row], s_L[row]);
     }
   }
-  if (wk.count > 1) join_parts(p, sp.parts, wk, kvh, row0, rows, ROWS, red);
+  if (wk.count > 1 && !sp.scores) join_parts(p, sp.parts, wk, kvh, row0, rows, ROWS, red);
 }
 
-// The weights of the stored scores (T = 1) added to the slots of a sequence,
-// four slots a thread: they need every head's log-sum, which no CTA of the
-// attention has before its end.  Reads back 4 bytes a head and slot, from L2;
-// 6 us alone, 2 to 3 behind the attention, under which it is launched.
-constexpr int kAdd = 128;
-
-__global__ void __launch_bounds__(kAdd) add_weights_kernel(const __grid_constant__ StreamParams sp) {
+// The second half of a decode step (T = 1), launched under the attention: a
+// sequence's first CTAs add the weights of the stored scores to its slots, four
+// slots a thread, the others join the outputs of its items.  The
+// weights need every head's log-sum, which no CTA of the attention has before
+// its end, so each CTA takes it from the parts' statistics: the attention ends
+// without a join of its own (51.0 us for 8 sequences of up to 32K slots, 9.0 for
+// one of 1000; with that join 52.8 and 12.0).  Reads back 4 bytes a head and slot, from L2.
+constexpr int kAdd = 256;
+__global__ void __launch_bounds__(kAdd) finish_decode_kernel(const __grid_constant__ StreamParams sp,
+                                                             int grid, int rows, int adds) {
+  __shared__ float s_z[128 * 16];  // log2 of the sum of exp(score), by head
   const TreeParams &p = sp.t;
-  const int b = blockIdx.y, x = (blockIdx.x * kAdd + threadIdx.x) * 4;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = blockIdx.y;
+  const int hd = p.kv.head_dim, G = p.n_heads / p.kv.kv_heads, H = p.n_heads;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // lens and acc come from before the attention, which writes neither
-  const int len = committed(p.kv, p.lens, b, 1);
-  if (x > len) return;
+  const int x = (blockIdx.x * kAdd + tid) * 4, len = committed(p.kv, p.lens, b, 1);
+  if ((int)blockIdx.x < adds && (int)blockIdx.x * kAdd * 4 > len) return;
+  Work wk;
+  find_work(p, kTile, p.kv.kv_heads * sp.blocks, whole_tiles(hd), lane, wk, grid, 0, b);
+  // a head's statistics: of part i at + i * rows
+  auto stat_of = [&](int h) {
+    const int kvh = quick_div(h, G), r = h - kvh * G, blk = quick_div(r, rows);
+    return (size_t)(wk.first + (kvh * sp.blocks + blk) * wk.count) * rows + (r - blk * rows);
+  };
+  if ((int)blockIdx.x >= adds) {  // ---- outputs
+    const int hd4 = hd / 4, per = kAdd / hd4, in = tid / hd4, d = tid - in * hd4;
+    const int h = ((int)blockIdx.x - adds) * per + in;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (in >= per || h >= H) return;
+    const size_t at = stat_of(h);
+    const float4 *part = reinterpret_cast<const float4 *>(sp.parts.part) + at * hd4 + d;
+    const Joined j = join_row4(sp.parts.stat + at, part, rows, (size_t)rows * hd4, wk.count);
+    reinterpret_cast<float4 *>(p.out + (size_t)b * p.out_ld + (size_t)h * hd)[d] = j.a;
+    return;
+  }
   float *acc = p.kv.acc + (size_t)b * p.kv.acc_stride + x;
   float old[4];
 #pragma unroll
   for (int k = 0; k < 4; k++) old[k] = x + k < len ? p.decay * acc[k] : 0.0f;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const float *lse = p.lse + (size_t)b * p.n_heads;
-  const float *s = sp.scores + (size_t)b * p.n_heads * sp.score_ld + x;
+  const float *s = sp.scores + (size_t)b * H * sp.score_ld + x;
+  constexpr int kHeads = 8;  // whose scores are on their way together
+  float4 v[kHeads];
+  auto load = [&](int h0) {
+#pragma unroll
+    for (int i = 0; i < kHeads; i++)
+      if (x <= len && h0 + i < H)
+        v[i] = *reinterpret_cast<const float4 *>(s + (size_t)(h0 + i) * sp.score_ld);
+  };
+  load(0);
+  for (int h = warp; h < H; h += kAdd / 32) {
+    const float2 *stat = sp.parts.stat + stat_of(h);
+    float M = -INFINITY, L = 0.0f;
+    for (int i0 = 0; i0 < wk.count; i0 += 32) {
+      const float2 w = i0 + lane < wk.count ? stat[(size_t)(i0 + lane) * rows]
+                                            : make_float2(-INFINITY, 0.0f);
+      const float N = fmaxf(M, warp_max(w.x)), ref = N == -INFINITY ? 0.0f : N;
+      L = L * ex2(M - ref) + w.y * ex2(w.x - ref);
+      M = N;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    if (lane == 0) s_z[h] = M + log2f(L);  // never empty: a token sees itself
+  }
+  __syncthreads();
   float sum[4] = {};
-#pragma unroll 8
-  for (int h = 0; h < p.n_heads; h++) {
-    const float4 v = *reinterpret_cast<const float4 *>(s + (size_t)h * sp.score_ld);
-    // an empty row cannot be: a token sees itself
-    const float z = lse[h] * kLog2e;
-    sum[0] += ex2(__fmaf_rn(v.x, kLog2e, -z));
-    sum[1] += ex2(__fmaf_rn(v.y, kLog2e, -z));
-    sum[2] += ex2(__fmaf_rn(v.z, kLog2e, -z));
-    sum[3] += ex2(__fmaf_rn(v.w, kLog2e, -z));
+  for (int h0 = 0; h0 < H; h0 += kHeads) {
+    if (h0 > 0) load(h0);
+#pragma unroll
+    for (int i = 0; i < kHeads; i++)
+      if (h0 + i < H) {
+        const float z = s_z[h0 + i];
+        sum[0] += ex2(__fmaf_rn(v[i].x, kLog2e, -z));
+        sum[1] += ex2(__fmaf_rn(v[i].y, kLog2e, -z));
+        sum[2] += ex2(__fmaf_rn(v[i].z, kLog2e, -z));
+        sum[3] += ex2(__fmaf_rn(v[i].w, kLog2e, -z));
+      }
   }
 #pragma unroll
   for (int k = 0; k < 4; k++)
@@ -484,7 +533,7 @@ void stream_blocks(const fgm_cuda_kv &kv, int n_heads, int T, int &nt, int &bloc
 }
 
 struct Ws {
-  size_t counters, part, stat, lse, scores, total;
+  size_t counters, part, stat, scores, total;
   int score_ld;
 };
 Ws ws_of(const fgm_cuda_kv &kv, int n_heads, int T) {
@@ -496,8 +545,7 @@ Ws ws_of(const fgm_cuda_kv &kv, int n_heads, int T) {
   w.counters = 0;
   w.part = kCounters * sizeof(int);
   w.stat = w.part + align256(grid * 8 * nt * kv.head_dim * sizeof(float));
-  w.lse = w.stat + align256(grid * 8 * nt * sizeof(float2));
-  w.scores = w.lse + align256((size_t)kv.rows * n_heads * sizeof(float));
+  w.scores = w.stat + align256(grid * 8 * nt * sizeof(float2));
   w.score_ld = (kv.cap + 31) & ~31;
   w.total = w.scores +
             (T == 1 ? align256((size_t)kv.rows * n_heads * w.score_ld * sizeof(float)) : 0);
@@ -528,11 +576,6 @@ cudaError_t launch_stream(const TreeParams &p, bool accumulate, int num_sms, cud
   sp.parts.counters = reinterpret_cast<int *>(ws + w.counters);
   sp.scores = accumulate ? reinterpret_cast<float *>(ws + w.scores) : nullptr;
   sp.score_ld = w.score_ld;
-  if (accumulate) {
-    sp.t.lse = reinterpret_cast<float *>(ws + w.lse);
-    sp.t.lse_row = (size_t)p.n_heads;
-    sp.t.lse_head = 1;
-  }
   cudaError_t e = cudaErrorInvalidValue;
   switch (p.kv.head_dim * 2 + nt - 1) {
     case 128: e = launch_stream_as<64, 1>(sp, grid, st); break;
@@ -549,8 +592,9 @@ cudaError_t launch_stream(const TreeParams &p, bool accumulate, int num_sms, cud
     case 1024: e = launch_stream_as<512, 1>(sp, grid, st); break;
   }
   if (e != cudaSuccess || !accumulate) return e;
+  const int adds = (p.kv.cap + 4 * kAdd - 1) / (4 * kAdd), per = kAdd / (p.kv.head_dim / 4);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((p.kv.cap + 4 * kAdd - 1) / (4 * kAdd)), (unsigned)p.kv.rows);
+  cfg.gridDim = dim3((unsigned)(adds + (p.n_heads + per - 1) / per), (unsigned)p.kv.rows);
   cfg.blockDim = dim3(kAdd);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -558,7 +602,7 @@ cudaError_t launch_stream(const TreeParams &p, bool accumulate, int num_sms, cud
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, add_weights_kernel, sp);
+  return cudaLaunchKernelEx(&cfg, finish_decode_kernel, sp, grid, 8 * nt, adds);
 }
 
 }  // namespace

@@ -521,8 +521,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Joins an item's partial results: a CTA takes a few rows, a thread four
-// dimensions of one.  The first parts' values are asked for together with
-// their statistics.
+// dimensions of one.
 constexpr int kJoin = 256;
 __global__ void __launch_bounds__(kJoin) tile_join_kernel(const __grid_constant__ TileParams tp,
                                                           int groups) {
@@ -542,39 +541,13 @@ __global__ void __launch_bounds__(kJoin) tile_join_kernel(const __grid_constant_
   if (de.y == 1) return;
   const float2 *stat = tp.stat + (size_t)de.x * kTM + row;
   const float4 *part = reinterpret_cast<const float4 *>(tp.part) + ((size_t)de.x * kTM + row) * dv4 + d;
-  float M = -INFINITY, L = 0.0f;
-  float4 a = make_float4(0, 0, 0, 0);
-  constexpr int kParts = 12;
-  for (int i0 = 0; i0 < de.y; i0 += kParts) {
-    float2 s[kParts];
-    float4 v[kParts];
-    const int n = min(kParts, de.y - i0);
-#pragma unroll
-    for (int i = 0; i < kParts; i++) {
-      s[i] = i < n ? stat[(size_t)(i0 + i) * kTM] : make_float2(-INFINITY, 0.0f);
-      v[i] = i < n ? part[(size_t)(i0 + i) * kTM * dv4] : make_float4(0, 0, 0, 0);
-    }
-    float N = M;
-#pragma unroll
-    for (int i = 0; i < kParts; i++) N = fmaxf(N, s[i].x);
-    const float ref = N == -INFINITY ? 0.0f : N, f0 = ex2(M - ref);
-    a.x *= f0, a.y *= f0, a.z *= f0, a.w *= f0;
-    L *= f0;
-#pragma unroll
-    for (int i = 0; i < kParts; i++) {
-      const float f = ex2(s[i].x - ref);
-      L += f * s[i].y;
-      a.x += f * v[i].x, a.y += f * v[i].y, a.z += f * v[i].z, a.w += f * v[i].w;
-    }
-    M = N;
-  }
-  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+  const Joined j = join_row4(stat, part, kTM, (size_t)kTM * dv4, de.y);
   const int node = r / G, h = kvh * G + r - node * G;
   const size_t qr = (size_t)b * p.T + node;
-  reinterpret_cast<float4 *>(p.out + qr * p.out_ld + (size_t)h * hd + ds * dv)[d] =
-      make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+  reinterpret_cast<float4 *>(p.out + qr * p.out_ld + (size_t)h * hd + ds * dv)[d] = j.a;
   if (d == 0 && ds == 0 && p.lse)
-    p.lse[qr * p.lse_row + h * p.lse_head] = L == 0.0f ? -INFINITY : (M + log2f(L)) * kLn2;
+    p.lse[qr * p.lse_row + h * p.lse_head] =
+        j.L == 0.0f ? -INFINITY : (j.M + log2f(j.L)) * kLn2;
 }
 
 constexpr int kMaxSmem = 210 * 1024;  // of any head_dim

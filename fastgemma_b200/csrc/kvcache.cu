@@ -432,22 +432,22 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictPar
   if (rank == 0 && tid == 0) p.lens_out[b] = budget;
 }
 
-// A warp per kMoveSlots slots of a sequence: the rows that move, their loads
+// A warp per `per` slots of a sequence: the rows that move, their loads
 // all on the way before the first store.  Rows move from past the budget to
 // below it, so no order matters.  Bound by memory latency and by sectors that
 // are read and written for one byte in four of V: 14336 rows of 512 dimensions
 // in 16 us.  Rows listed per CTA of 64 slots before they move took 18.7, whole
 // words of V, merged and stored, 19.7, the rows past the budget asked for in L2
 // during the plan 16.6.
-constexpr int kMoveSlots = 8, kMoveWarps = 8;
+constexpr int kMoveWarps = 4;
 __global__ void __launch_bounds__(kMoveWarps * 32) evict_move_kernel(const EvictParams p,
-                                                                     int groups) {
+                                                                     int groups, int per) {
   const int item = blockIdx.x * kMoveWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int b = item / groups, x0 = (item - b * groups) * kMoveSlots;
+  const int b = item / groups, x0 = (item - b * groups) * per;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (b >= p.kv.rows) return;
   const int x = x0 + lane, kvd = p.kv.kv_heads * p.kv.head_dim;
-  const int s = lane < kMoveSlots && x < p.budget ? p.map[(size_t)b * p.budget + x] : -1;
+  const int s = lane < per && x < p.budget ? p.map[(size_t)b * p.budget + x] : -1;
   unsigned todo = __ballot_sync(0xffffffffu, s >= 0 && s != x);
   int8_t *kc = p.kv.kc + (size_t)b * p.kv.kc_stride, *vt = p.kv.vt + (size_t)b * p.kv.vt_stride;
   float *ks = p.kv.ks + (size_t)b * p.kv.ks_stride, *vs = p.kv.vs + (size_t)b * p.kv.vs_stride;
@@ -545,7 +545,13 @@ cudaError_t launch_kv_evict(const fgm_cuda_kv &kv, const int32_t *lens, int budg
   cfg.blockDim = dim3(kPlanThreads);
   cfg.dynamicSmemBytes = (size_t)words * 8 + (size_t)(cached ? words : (words + 1) / 2) * 128;
   if ((e = cudaLaunchKernelEx(&cfg, plan, p)) != cudaSuccess) return e;
-  const int groups = (budget + kMoveSlots - 1) / kMoveSlots;
+  // Slots of a warp that moves rows: one while about all warps fit the SMs at
+  // once, more to spare launches of CTAs that find nothing.  One, two, four: 6.4,
+  // 7.0, 7.5 us at 512 slots in all, 7.1, 7.5, 8.2 at 4096, 16.0, 15.7, 16.2 at
+  // 14400, 18.6, 17.5, 17.5 at 28800, 35.5, 30.9, 29.9 at 114688.
+  const long long slots = (long long)kv.rows * budget;
+  const int per = slots <= 8192 ? 1 : slots <= 32768 ? 2 : 4;
+  const int groups = (budget + per - 1) / per;
   const long long items = (long long)kv.rows * groups;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -553,7 +559,7 @@ cudaError_t launch_kv_evict(const fgm_cuda_kv &kv, const int32_t *lens, int budg
   cfg.dynamicSmemBytes = 0;
   cfg.gridDim = dim3((unsigned)((items + kMoveWarps - 1) / kMoveWarps));
   cfg.blockDim = dim3(kMoveWarps * 32);
-  return cudaLaunchKernelEx(&cfg, evict_move_kernel, p, groups);
+  return cudaLaunchKernelEx(&cfg, evict_move_kernel, p, groups, per);
 }
 
 }  // namespace fgm

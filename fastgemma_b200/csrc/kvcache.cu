@@ -184,22 +184,23 @@ __device__ __forceinline__ uint32_t rank_key(float v) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// A cluster of CTAs per sequence, a run of slots each.  The budget-th largest
+// One CTA per sequence over caches of up to kOneCta slots, else a cluster of
+// kCluster, a run of slots each.  The budget-th largest
 // key comes from passes of 256 counters over its bytes, summed over the cluster
 // through distributed shared memory, until the keys that share the bytes so far
 // all stay (`exact`) or the four bytes are known; then every warp walks its
 // share of the run, 32 slots at a time, and leaves the kept ones as a bitmask
 // with the number kept before each word.  Each CTA lists its kept slots past
 // the budget (where the keys were); the evicted slots below it find their
-// sources there, by rank over the lists.  Bound by latency: a cluster barrier
-// and a pass or two over the slots for each of six to nine steps, which is why
-// a run is short (kRunSlots) and its keys stay in shared memory (CACHED; longer
-// runs read acc and tpos again in every pass).  8 sequences of 16K slots: 15.8
-// us (with one CTA a sequence about 20 more), of which 2.3 until the keys are there, 1.5
-// for each barrier with its counters, 3.2 for the map; 600 slots: 6.
-constexpr int kRunSlots = 2048, kCachedKeys = 40960;
-
-constexpr int kMaxCluster = 8;
+// sources there, by rank over the lists.  Bound by latency: a barrier and a pass
+// or two over the slots for each of six to nine steps, which is why the keys stay
+// in shared memory (CACHED; longer runs read acc and tpos again in every pass).
+// 8 sequences of 16K slots: 15.8 us (with one CTA each about 20 more), of which
+// 2.3 until the keys are there, 1.5 for each barrier with its counters, 3.2 for
+// the map; 600 slots in one CTA: 6.  With the moves, one CTA against clusters of
+// two, four and eight: 10.3, 14.2, 12.7 and 12.9 us at 4096 slots; 14.6 against
+// 16.9, 14.6 and 13.9 at 8000.
+constexpr int kOneCta = 6144, kCluster = 8, kCachedKeys = 40960;
 
 template <bool CACHED, bool CLUSTER>
 __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictParams p) {
@@ -209,7 +210,7 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictPar
   __shared__ uint32_t s_prefix;
   __shared__ int s_left, s_exact;
   cg::cluster_group cluster = cg::this_cluster();
-  const int C = CLUSTER ? (int)cluster.num_blocks() : 1;
+  constexpr int C = CLUSTER ? kCluster : 1;
   const int rank = CLUSTER ? (int)cluster.block_rank() : 0;
   auto sync = [&] {
     if (CLUSTER) cluster.sync();
@@ -242,11 +243,10 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictPar
   uint32_t *bits = smem, *before = smem + words, *keys = before + words;
   // kept slots past the budget, from the run's first; a run has at most 65536
   uint16_t *list = reinterpret_cast<uint16_t *>(keys);
-  // a word of every CTA of the cluster, all asked for at once (0 past the last)
-  auto all = [&](int *w, int (&v)[kMaxCluster]) {
+  // a word of every CTA of the cluster, all asked for at once
+  auto all = [&](int *w, int (&v)[C]) {
 #pragma unroll
-    for (int r = 0; r < kMaxCluster; r++)
-      v[r] = !CLUSTER ? (r == 0 ? *w : 0) : r < C ? *cluster.map_shared_rank(w, r) : 0;
+    for (int r = 0; r < C; r++) v[r] = CLUSTER ? *cluster.map_shared_rank(w, r) : *w;
   };
 
   // the newest position (the slot's index where no positions are kept)
@@ -267,12 +267,10 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictPar
     newest = __reduce_max_sync(0xffffffffu, newest);
     if (lane == 0) atomicMax(&s_newest, newest);
     sync();
-    int v[kMaxCluster];
+    int v[C];
     all(&s_newest, v);
-    newest = v[0];
 #pragma unroll
-    for (int r = 1; r < kMaxCluster; r++)
-      if (r < C) newest = max(newest, v[r]);
+    for (int r = 0; r < C; r++) newest = max(newest, v[r]);
   }
   const long long old = (long long)newest - p.recent;
   auto make_key = [&](int x) -> uint32_t {
@@ -296,9 +294,12 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictPar
     }
     sync();
     if (tid < 256) {
-      int v[kMaxCluster];
+      int v[C];
       all(reinterpret_cast<int *>(&hist[pass][tid]), v);
-      total[tid] = (unsigned)(((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7])));
+      unsigned sum = 0;
+#pragma unroll
+      for (int r = 0; r < C; r++) sum += (unsigned)v[r];
+      total[tid] = sum;
     }
     __syncthreads();
     if (warp == 0) {  // the digit, from the largest down: 8 counters a lane
@@ -355,7 +356,7 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictPar
     }
     return sum;  // of thread 0
   };
-  int v[kMaxCluster], lows[kMaxCluster];
+  int v[C], lows[C];
   int seen = 0;  // equal keys before this warp's
   if (!exact) {
     int count = 0;
@@ -369,7 +370,7 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictPar
     seen = s_warp[warp];
     all(&s_eq, v);
 #pragma unroll
-    for (int r = 0; r < kMaxCluster; r++)
+    for (int r = 0; r < C; r++)
       if (r < rank) seen += v[r];
     __syncthreads();
   }
@@ -409,7 +410,7 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictPar
   all(&s_kept, v);
   all(&s_kept_low, lows);
 #pragma unroll
-  for (int r = 0; r < kMaxCluster; r++)
+  for (int r = 0; r < C; r++)
     if (r < rank) base += v[r];
   for (int x = first + tid; x < min(last, budget); x += kPlanThreads) {
     const int w = (x - first) >> 5;
@@ -418,7 +419,7 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictPar
     if (!(word & bit)) {  // as many evicted slots lie before it as kept ones before its source
       int i = x - (base + (int)before[w] + __popc(word & (bit - 1))), from = 0;
 #pragma unroll
-      for (int r = 0; r < kMaxCluster - 1; r++)
+      for (int r = 0; r < C - 1; r++)
         if (from == r && i >= v[r] - lows[r]) {
           i -= v[r] - lows[r];
           from++;
@@ -521,9 +522,7 @@ cudaError_t launch_kv_evict(const fgm_cuda_kv &kv, const int32_t *lens, int budg
                 out_stride};
   if (!acc_out) p.acc_out = kv.acc, p.acc_stride = kv.acc_stride;
   if (!tpos_out) p.tpos_out = kv.tpos, p.tpos_stride = kv.tpos_stride;
-  // CTAs of a sequence: runs of about kRunSlots, at most a cluster of 8
-  int c = 1;
-  while (c < kMaxCluster && kv.cap > c * kRunSlots) c <<= 1;
+  const int c = kv.cap <= kOneCta ? 1 : kCluster;
   const int words = ((kv.cap + c - 1) / c + 31) / 32;
   // the keys' room also takes the list of kept slots past the budget, which
   // has no more entries than there are evicted ones

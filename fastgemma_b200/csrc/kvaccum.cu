@@ -10,7 +10,7 @@
 // buffers keep the tensor cores ahead of the exponentials: one per (query row,
 // slot) pair at 16 a cycle per SM.
 //
-// 256 nodes, 8 heads over 2, over 16K slots of head_dim 256: 25.8 us, 34 M
+// 256 nodes, 8 heads over 2, over 16K slots of head_dim 256: 25.5 us, 34 M
 // exponentials (the exponential unit 42 % busy, 8.2 us alone; without any
 // arithmetic on the scores 20.6, without masks 22.8).  A launch is one tile of
 // slots per CTA, so what is left is the start of each: the quantisation before
@@ -25,8 +25,8 @@ namespace {
 
 using namespace kv;
 
-constexpr int kAddWarps = 16, kAdd = kAddWarps * 32;
-constexpr int kThreads = 128 + kAdd;
+constexpr int kAddWarps = 16;
+constexpr int kThreads = 128 + kAddWarps * 32;
 constexpr int kQuarter = 32;     // query rows of a thread per block
 constexpr int kBufs = 4;         // score buffers of 128 TMEM columns
 constexpr int kQStages = 6;      // ring of 16 KB query chunks
@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < kBufs; i++) {
       tc::mbar_init(&bar.c_full[i], 1);
       tc::mbar_init(&bar.d_full[i], 1);
-      tc::mbar_init(&bar.d_empty[i], kAdd);
+      tc::mbar_init(&bar.d_empty[i], kAddWarps);
     }
     tc::fence_mbar_init();
     s_abort = 0;
@@ -297,7 +297,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
             tc::fence_before_sync();
-            tc::mbar_arrive(&bar.d_empty[buf]);
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&bar.d_empty[buf]);
           }
       }
       s_sum[t & 1][quarter][in_tile] = sum;

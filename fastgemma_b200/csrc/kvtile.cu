@@ -130,13 +130,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::mbar_init(&bar.k_empty[i], 1);
     }
     for (int i = 0; i < kVStages; i++) {
-      tc::mbar_init(&bar.v_full[i], 128);
+      tc::mbar_init(&bar.v_full[i], 4);
       tc::mbar_init(&bar.v_empty[i], 1);
     }
     for (int i = 0; i < 2; i++) {
-      tc::mbar_init(&bar.p_full[i], kSoft / 2);
+      tc::mbar_init(&bar.p_full[i], kSoftWarps / 2);
       tc::mbar_init(&bar.p_empty[i], 1);
-      tc::mbar_init(&bar.sc_full[i], 32);
+      tc::mbar_init(&bar.sc_full[i], 1);
       tc::mbar_init(&bar.sc_empty[i], kSoftWarps);
     }
     tc::mbar_init(&bar.q_full, 1);
@@ -192,7 +192,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         s_ks[j & 1][lane + 32 * k] = a[k];
         s_vs[j & 1][lane + 32 * k] = c[k];
       }
-      tc::mbar_arrive(&bar.sc_full[j & 1]);
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&bar.sc_full[j & 1]);
     }
   } else if (warp == 1) {  // ---- MMAs
     // descriptors differ from these in their address field, 16 bytes a unit
@@ -300,7 +301,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (h + 1 < halves) load(h + 1);
       stream::fence_proxy_async_smem();
-      tc::mbar_arrive(&bar.v_full[st]);
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&bar.v_full[st]);
       if (++st == kVStages) st = 0, ph ^= 1;
     }
   } else if (warp >= 4) {  // ---- softmax: row (warp % 4) * 32 + lane, slots 32 * quarter ...
@@ -453,9 +455,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         tile(j, std::false_type());
       }
       tc::fence_before_sync();
-      tc::mbar_arrive(&bar.p_full[quarter >> 1]);
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&bar.sc_empty[j & 1]);
+      if (lane == 0) {
+        tc::mbar_arrive(&bar.p_full[quarter >> 1]);
+        tc::mbar_arrive(&bar.sc_empty[j & 1]);
+      }
     }
     // ---- results: the quarters' sums joined, each quarter's dimensions to
     // shared memory, whole rows from there (what the loads filled is free now)

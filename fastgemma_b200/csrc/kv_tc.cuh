@@ -150,9 +150,10 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 // Waits until the phase with `parity` is over.  The tests put the warp to sleep
 // for up to 10 us each: spinning, or reading a clock or the abort word between
 // the tests, takes issue slots from the warps that work (256 nodes over 16K
-// slots 65.7 us like this, 68.9 when the MMA warp alone spins, 71 when all do).  After kWaitTests tests, two seconds asleep,
-// the wait gives up and raises the abort word, on which later waits do not
-// sleep any more: the loops run out, the CTA reports and leaves.
+// slots 65.7 us like this, 68.9 when the MMA warp alone spins, 71 when all do).
+// After kWaitTests tests, two seconds asleep, the wait gives up and raises the
+// abort word, on which later waits do not sleep any more: the loops run out,
+// the CTA reports and leaves.
 constexpr int kWaitTests = 200000;
 __device__ __forceinline__ void wait_phase(uint64_t *bar, uint32_t parity, int *abort) {
   if (tc::mbar_try_wait(bar, parity)) return;

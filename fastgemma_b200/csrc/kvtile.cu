@@ -401,6 +401,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_st_x8(quad + c, o);
         }
         tmem_wait_st();
+        // A half's product adds into all of the output's columns, but waits for
+        // the weights of two quarters alone, so nobody hands over weights before
+        // all four have stored.  (They see the same maxima and get here
+        // together.)  It also keeps every quarter within one phase of p_empty
+        // of both halves, which a wait by parity needs.
+        tc::fence_before_sync();
+        meet();
+        tc::fence_after_sync();
       }
       const float ref = m == -INFINITY ? 0.0f : m;
       const uint64_t qs2 = pair2(qs, qs), ref2 = pair2(-ref, -ref), minus = pair2(-1.0f, -1.0f);

@@ -1,0 +1,53 @@
+"""The KV-cache operators where their kernels divide or reorder the work in
+ways that short random cases do not reach.  Helpers, caches and tolerances are
+those of test_kv_tree.py."""
+import numpy as np
+import pytest
+
+import fastgemma_b200.device as D
+from test_kv_tree import EPS, Cache, check_attend, dev, run_attend
+
+torch = pytest.importorskip("torch")
+gpu = pytest.mark.gpu
+
+
+# ------------------------------------- maxima that grow all along a long run
+def staircases(rng, rows, T, H, kvh, hd, tiles):
+    """Scores by tile of 128 slots: a query row's rises by 7 levels a tile up
+    to a tile of its own and stays there.  K holds 127 in the dimension of the
+    slot's tile, q the row's level there (and 127 where K holds 0, which makes
+    the int8 query the levels themselves), and a level is 9 ln 2 / 7, so that
+    one step multiplies the weights by 2^9."""
+    n = tiles * 128 - T
+    cache = Cache(rng, rows, n + T, kvh, hd)
+    k = cache.k.reshape(rows, n + T, kvh, hd)
+    k[..., :tiles] = k[..., -1:] = 0
+    for x in range(n + T):
+        k[:, x, :, x // 128] = 127
+    cache.ks[:] = 9 * np.log(2) / 7 / 127 * rng.uniform(0.99, 1.01, cache.ks.shape)
+    level = np.arange(tiles) * 7
+    stop = (np.arange(rows * T * H) * 5 % tiles).reshape(rows * T, H)
+    q = np.zeros((rows * T, H, hd), np.float32)
+    q[..., :tiles] = np.minimum(level, level[stop][..., None])
+    q[..., -1] = 127
+    pos = np.tile(n + np.arange(T, dtype=np.int32), (rows, 1))
+    return cache, q.reshape(rows * T, -1), [n] * rows, pos
+
+
+@gpu
+@pytest.mark.parametrize("rows,T,H,kvh,hd,tiles", [(16, 16, 64, 8, 64, 16),  # a CTA an item
+                                                   (16, 64, 8, 4, 256, 16),
+                                                   (3, 33, 16, 4, 320, 17),
+                                                   (8, 128, 4, 4, 512, 16),
+                                                   (37, 20, 4, 4, 128, 16)])
+def test_maxima_that_grow_in_every_tile(rows, T, H, kvh, hd, tiles):
+    """In every tile some rows of each warp rescale their output and others
+    keep all that it holds: the rescaling has to come before the products."""
+    rng = np.random.default_rng(hd)
+    cache, q, lens, pos = staircases(rng, rows, T, H, kvh, hd, tiles)
+    (kv, qd, ld, _, pd, out, lse), _, _ = check_attend(cache, q, H, T, lens, None, pos, 0)
+    ws = D.attend_workspace(kv, H, T)
+    again, lse2 = torch.empty_like(qd), torch.empty_like(lse)
+    for _ in range(50):
+        D.attend_tree_q8(again, qd, kv, H, T, ld, pos=pd, lse=lse2, ws=ws)
+        assert torch.equal(again, out) and torch.equal(lse2, lse)

@@ -332,8 +332,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 // A warp per query row of a block of 128: its int8 copy in the block's
 // swizzled place and its scale; 4 us for any size in use, of which the kernel
 // after it, launched early, spends 3 on its own setup.  For the attention the scale times log2(e);
-// for the accumulation (p.decay in use, cst set) the scale itself and -lse,
-// -infinity where a row adds nothing.
+// for the accumulation (p.decay in use, cst set) the scale itself and -lse, 0
+// and -infinity where a row adds nothing.
 constexpr int kQuantRows = 8;
 __global__ void __launch_bounds__(kQuantRows * 32)
     quant_rows_kernel(const __grid_constant__ TreeParams p, int blocks, int nkb, int8_t *q8,
@@ -377,7 +377,9 @@ __global__ void __launch_bounds__(kQuantRows * 32)
   if (cst) {
     const float lse = p.lse[qr * p.lse_row + h * p.lse_head];
     const bool adds = lse != -INFINITY && (!p.take || p.take[qr]);
-    cst[(size_t)block * 2 * kTM + j] = q_scale(top);
+    // no scale either where it adds nothing: one that is no number would make
+    // the constant -infinity no number
+    cst[(size_t)block * 2 * kTM + j] = adds ? q_scale(top) : 0.0f;
     cst[(size_t)block * 2 * kTM + kTM + j] = adds ? -lse : -INFINITY;
   } else {
     // never 0, so that a masked score stays -inf (a zero query's dots are 0)

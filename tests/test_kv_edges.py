@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import fastgemma_b200.device as D
-from test_kv_tree import EPS, Cache, check_attend, dev, run_attend
+from test_kv_tree import Cache, check_attend, dev, run_attend, setup
 
 torch = pytest.importorskip("torch")
 gpu = pytest.mark.gpu
@@ -51,3 +51,27 @@ def test_maxima_that_grow_in_every_tile(rows, T, H, kvh, hd, tiles):
     for _ in range(50):
         D.attend_tree_q8(again, qd, kv, H, T, ld, pos=pd, lse=lse2, ws=ws)
         assert torch.equal(again, out) and torch.equal(lse2, lse)
+
+
+# ------------------------------------------------- nodes that add nothing
+@gpu
+@pytest.mark.parametrize("T,H,kvh,hd,kind", [(2, 4, 2, 64, "chain"), (48, 8, 2, 128, "tree"),
+                                             (150, 4, 2, 320, "chain")])
+def test_a_node_that_is_not_taken_adds_nothing_whatever_its_query_holds(T, H, kvh, hd, kind):
+    """Rejected nodes with a not-a-number and an infinity in a query head: the
+    slots' weights have the bits they have with finite queries there."""
+    rng = np.random.default_rng(T)
+    lens = [300, 77]
+    cache, q, mask, pos = setup(rng, lens, T, H, kvh, hd, kind)
+    take = rng.integers(0, 2, (2, T)).astype(np.uint8)
+    take[:, 1], take[:, 0] = 0, 1
+    got = []
+    for bad in (False, True):
+        if bad:
+            q[1, 3] = np.nan
+            q[T + 1, hd:] = np.inf
+        kv, qd, ld, w, pd, _, lse = run_attend(cache, q, H, T, lens, mask, pos, 0)
+        D.attend_accum_q8(qd, kv, H, T, ld, lse, mask=w, pos=pd, take=dev(take), decay=0.5)
+        got.append(cache.d["acc"].cpu().numpy())
+    assert np.isfinite(got[0]).all()
+    assert np.array_equal(got[0].view(np.uint32), got[1].view(np.uint32))

@@ -274,8 +274,23 @@ def _flat(**tensors):
                              f"{t.stride()}")
 
 
-def _lse(lse):
-    return (None, 0, 0) if lse is None else (lse.data_ptr(), lse.stride(0), lse.stride(1))
+def _rows(**tensors):
+    """The same for rows of f32 at a distance the caller gives."""
+    for name, t in tensors.items():
+        if t is not None and (t.dtype != torch.float32 or
+                              (t.shape[-1] > 1 and t.stride(-1) != 1)):
+            raise ValueError(f"{name} has to be torch.float32 with its last dimension contiguous, "
+                             f"not {t.dtype} with strides {t.stride()}")
+
+
+def _lse(lse, rows, n_heads):
+    if lse is None:
+        return None, 0, 0
+    if (lse.dtype != torch.float32 or lse.dim() != 2 or lse.shape[0] < rows or
+            lse.shape[1] < n_heads):
+        raise ValueError(f"lse: {lse.dtype} {tuple(lse.shape)}, need torch.float32 of "
+                         f"[{rows}][{n_heads}]")
+    return lse.data_ptr(), lse.stride(0), lse.stride(1)
 
 
 def _on(stream):
@@ -311,11 +326,13 @@ def attend_tree_q8(out, q, kv, n_heads, T, lens, mask=None, pos=None, window=0, 
     """T nodes of each sequence attend to its cache and to one another (mask
     None: to the nodes before them); lse [rows * T][n_heads], of any strides, if wanted."""
     _flat(lens=lens, mask=mask, pos=pos)
+    _rows(q=q, out=out)
+    lse = _lse(lse, kv.rows * T, n_heads)
     ws = _ws(ws, kv, n_heads, T, stream)
     ld = n_heads * kv.head_dim
     call("fgm_cuda_attend_tree_q8", C.byref(kv), _p(q), ld if q_ld is None else q_ld, n_heads, T,
          _p(lens), _p(mask), _p(pos), window, _p(out), ld if out_ld is None else out_ld,
-         *_lse(lse), _p(ws), ws.numel(), _s(stream))
+         *lse, _p(ws), ws.numel(), _s(stream))
 
 
 def attend_accum_q8(q, kv, n_heads, T, lens, lse, mask=None, pos=None, window=0, take=None,
@@ -323,16 +340,19 @@ def attend_accum_q8(q, kv, n_heads, T, lens, lse, mask=None, pos=None, window=0,
     """kv's acc = decay * acc + the weights of the taken nodes (take: uint8
     [rows * T]) of such an attention, from its lse."""
     _flat(lens=lens, mask=mask, pos=pos, take=take)
+    _rows(q=q)
+    lse = _lse(lse, kv.rows * T, n_heads)
     ws = _ws(ws, kv, n_heads, T, stream)
     call("fgm_cuda_attend_accum_q8", C.byref(kv), _p(q),
          n_heads * kv.head_dim if q_ld is None else q_ld, n_heads, T, _p(lens), _p(mask), _p(pos),
-         window, *_lse(lse), _p(take), decay, _p(ws), ws.numel(), _s(stream))
+         window, *lse, _p(take), decay, _p(ws), ws.numel(), _s(stream))
 
 
 def attend_acc_q8(out, q, kv, n_heads, lens, decay=1.0, ws=None, q_ld=None, out_ld=None,
                   stream=None):
     """One token per sequence: attention over slots [0, lens[b]] and its weights added to kv's acc."""
     _flat(lens=lens)
+    _rows(q=q, out=out)
     ws = _ws(ws, kv, n_heads, 1, stream)
     ld = n_heads * kv.head_dim
     call("fgm_cuda_attend_acc_q8", C.byref(kv), _p(q), ld if q_ld is None else q_ld, n_heads,
@@ -363,6 +383,11 @@ def kv_evict_q8(kv, lens, budget, sink, recent, slot_map, lens_out, acc_out=None
     """Keep `budget` slots of each cache (protected, then by accumulated
     weight); slot_map [rows][budget] says where each slot's row came from."""
     _flat(lens=lens, slot_map=slot_map, lens_out=lens_out)
+    for name, t, dtype in (("acc_out", acc_out, torch.float32), ("tpos_out", tpos_out, torch.int32)):
+        if t is not None and (t.dtype != dtype or t.dim() != 2 or t.shape[0] < kv.rows or
+                              t.shape[1] < budget or (t.shape[1] > 1 and t.stride(1) != 1)):
+            raise ValueError(f"{name}: {t.dtype} {tuple(t.shape)} with strides {t.stride()}, need "
+                             f"{dtype} of [{kv.rows}][{budget}] with contiguous rows")
     stride = (acc_out if acc_out is not None else tpos_out).stride(0) \
         if acc_out is not None or tpos_out is not None else 0
     if acc_out is not None and tpos_out is not None and tpos_out.stride(0) != stride:
@@ -375,6 +400,7 @@ def qkv_post_tree(kv, q, k, v, n_heads, T, q_norm, k_norm, eps, inv_freq, pos, l
                   kv_ld=None, cs=None, stream=None):
     """qkv_post for the nodes of a tree: rope at pos, K / V rows into slots lens[b] + i."""
     _flat(pos=pos, lens=lens)
+    _rows(q=q, k=k, v=v)
     kvd = kv.kv_heads * kv.head_dim
     call("fgm_cuda_qkv_post_tree", C.byref(kv), _p(q),
          n_heads * kv.head_dim if q_ld is None else q_ld, _p(k), _p(v),

@@ -75,3 +75,43 @@ def test_a_node_that_is_not_taken_adds_nothing_whatever_its_query_holds(T, H, kv
         got.append(cache.d["acc"].cpu().numpy())
     assert np.isfinite(got[0]).all()
     assert np.array_equal(got[0].view(np.uint32), got[1].view(np.uint32))
+
+
+# --------------------------------------- tensors that would be misread
+def test_rows_of_another_type_or_stride_are_refused():
+    T, H, kvh, hd, cap = 3, 4, 2, 64, 12
+    kc, s = torch.zeros(2, cap, kvh * hd, dtype=torch.int8), torch.zeros(2, cap)
+    kv = D.KvCache(kc, s, kc.reshape(2, -1), s, kvh, hd, acc=torch.zeros(2, cap))
+    lens = torch.zeros(2, dtype=torch.int32)
+    q, ws = torch.zeros(2 * T, H * hd), torch.zeros(1, dtype=torch.uint8)
+    lse, one = torch.zeros(2 * T, H), torch.zeros(2, H * hd)
+
+    def refused(name, f, *a, **kw):
+        with pytest.raises(ValueError, match=name):
+            f(*a, ws=ws, **kw)
+
+    for bad in (q.bfloat16(), q.double(), torch.zeros(2 * T, H * hd, 2)[..., 0]):
+        refused("^q ", D.attend_tree_q8, q, bad, kv, H, T, lens)
+        refused("^out ", D.attend_tree_q8, bad, q, kv, H, T, lens)
+        refused("^q ", D.attend_accum_q8, bad, kv, H, T, lens, lse)
+        refused("^q ", D.attend_acc_q8, one, bad[:2], kv, H, lens)
+        refused("^out ", D.attend_acc_q8, bad[:2], one, kv, H, lens)
+    for bad in (lse.double(), lse.half(), lse[:5], lse[:, :3], lse.reshape(2, T, H), lse.flatten()):
+        refused("^lse", D.attend_tree_q8, q, q, kv, H, T, lens, lse=bad)
+        refused("^lse", D.attend_accum_q8, q, kv, H, T, lens, bad)
+
+    m = torch.zeros(2, 8, dtype=torch.int32)
+    acc, tpos = torch.zeros(2, 8), torch.zeros(2, 8, dtype=torch.int32)
+    for bad in (acc.double(), tpos, acc[:1], acc[:, :7], acc.flatten(), torch.zeros(8, 2).t(),
+                torch.zeros(2, 16)[:, ::2]):
+        with pytest.raises(ValueError, match="^acc_out"):
+            D.kv_evict_q8(kv, lens, 8, 1, 1, m, lens, acc_out=bad)
+    for bad in (tpos.long(), acc, tpos[:1], tpos[:, :7]):
+        with pytest.raises(ValueError, match="^tpos_out"):
+            D.kv_evict_q8(kv, lens, 8, 1, 1, m, lens, tpos_out=bad)
+
+    k, pos = torch.zeros(2 * T, kvh * hd), torch.zeros(2 * T, dtype=torch.int32)
+    w = torch.zeros(hd)
+    for name, a in (("q", (q.double(), k, k)), ("k", (q, k.half(), k)), ("v", (q, k, k.bfloat16()))):
+        with pytest.raises(ValueError, match=f"^{name} "):
+            D.qkv_post_tree(kv, *a, H, T, w, w, 1e-6, w, pos, lens)

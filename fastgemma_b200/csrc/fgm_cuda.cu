@@ -1902,7 +1902,7 @@ int fgm_cuda_qkv_post_tree(const fgm_cuda_kv *kv, float *q, int q_ld, float *k, 
   if (kv->ring && T > kv->ring)
     return fail(FGM_CUDA_EINVAL, "qkv_post_tree: T=%d ring=%d", T, kv->ring);
   if (kv->rows == 0) return FGM_CUDA_OK;
-  if (!q || !k || !v || !q_norm || !k_norm || !inv_freq || !pos || !lens)
+  if (!q || !k || !v || !q_norm || !k_norm || !inv_freq || !lens)
     return fail(FGM_CUDA_EINVAL, "qkv_post_tree: null pointer");
   if ((addr(q) | addr(k) | addr(v)) & 15)
     return fail(FGM_CUDA_EINVAL, "qkv_post_tree: q, k and v must be 16-byte aligned");

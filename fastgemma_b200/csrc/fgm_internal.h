@@ -142,7 +142,7 @@ struct QkvParams {
   const float *q_norm, *k_norm;     // [head_dim]
   float eps;
   const float *inv_freq;            // [head_dim / 2]
-  const int *pos;                   // [rows]
+  const int *pos;                   // [rows] (null: the slot's position, lens set)
   int ring;                         // 0: slot = pos, else pos % ring
   int cap;                          // cache slots per row
   int8_t *kc;

@@ -1035,7 +1035,8 @@ __global__ void __launch_bounds__(kGlueThreads) qkv_post_kernel(const QkvParams 
   float *qr = p.q + (size_t)r * p.q_ld, *kr = p.k + (size_t)r * p.kv_ld,
         *vr = p.v + (size_t)r * p.kv_ld;
   float *cs = xs + nq + 2 * kvd, *sn = cs + half, *qn = sn + half, *kn = qn + hd;
-  const int pos = p.pos[r];
+  const int c = r / p.T;  // its cache; the nodes of a tree share one
+  const int pos = p.pos ? p.pos[r] : p.lens[c] + (r - c * p.T);
   {  // q, k and v rows as float4, every load of a batch before any shared store
     const int q4 = nq >> 2, k4 = kvd >> 2, tot = q4 + 2 * k4;
     float4 *x4 = reinterpret_cast<float4 *>(xs);
@@ -1110,7 +1111,6 @@ __global__ void __launch_bounds__(kGlueThreads) qkv_post_kernel(const QkvParams 
     }
   }
   // int8 K and V rows with one scale each (ops.c:181-204), into the caches
-  const int c = r / p.T;  // its cache; the nodes of a tree share one
   const int at = p.lens ? p.lens[c] + (r - c * p.T) : pos;
   const int slot = p.ring ? at % p.ring : at;
   if (slot < 0 || slot >= p.cap) return;  // no cache entry for this row (whole CTA)

@@ -398,7 +398,8 @@ def kv_evict_q8(kv, lens, budget, sink, recent, slot_map, lens_out, acc_out=None
 
 def qkv_post_tree(kv, q, k, v, n_heads, T, q_norm, k_norm, eps, inv_freq, pos, lens, q_ld=None,
                   kv_ld=None, cs=None, stream=None):
-    """qkv_post for the nodes of a tree: rope at pos, K / V rows into slots lens[b] + i."""
+    """qkv_post for the nodes of a tree: rope at pos (None: at lens[b] + i), K / V rows into
+    slots lens[b] + i."""
     _flat(pos=pos, lens=lens)
     _rows(q=q, k=k, v=v)
     kvd = kv.kv_heads * kv.head_dim

@@ -556,9 +556,9 @@ int fgm_cuda_kv_evict_q8(const fgm_cuda_kv *kv, const int32_t *lens, int budget,
                          int32_t *tpos_out, size_t out_stride, void *stream);
 
 /* fgm_cuda_qkv_post_cs for the nodes of a tree: rows b*T + i of q, k and v
- * with rope at pos[b*T + i], the K / V rows into sequence b's cache at the
- * slot of position lens[b] + i (and kv->tpos there, when set).  A row whose
- * slot falls outside [0, cap) writes no cache entry. */
+ * with rope at pos[b*T + i] (pos NULL: at lens[b] + i), the K / V rows into
+ * sequence b's cache at the slot of position lens[b] + i (and kv->tpos there,
+ * when set).  A row whose slot falls outside [0, cap) writes no cache entry. */
 int fgm_cuda_qkv_post_tree(const fgm_cuda_kv *kv, float *q, int q_ld, float *k, float *v, int kv_ld,
                            int n_heads, int T, const float *q_norm, const float *k_norm, float eps,
                            const float *inv_freq, const float *cs, int positions,

@@ -115,3 +115,62 @@ def test_rows_of_another_type_or_stride_are_refused():
     for name, a in (("q", (q.double(), k, k)), ("k", (q, k.half(), k)), ("v", (q, k, k.bfloat16()))):
         with pytest.raises(ValueError, match=f"^{name} "):
             D.qkv_post_tree(kv, *a, H, T, w, w, 1e-6, w, pos, lens)
+
+
+# ------------------------------------------------ nodes into the cache
+@gpu
+@pytest.mark.parametrize("lens,T,H,kvh,hd,ring,q_pad,kv_pad", [
+    ([0], 1, 1, 1, 64, 0, 0, 0), ([50, 0, 37], 7, 8, 2, 256, 0, 12, 4), ([61, 10], 33, 4, 4, 128, 0, 0, 8),
+    ([100, 3], 20, 8, 1, 512, 33, 4, 0), ([9], 256, 16, 2, 192, 0, 0, 0),
+    ([1000, 40], 40, 12, 3, 320, 40, 8, 8)])
+def test_chain_rows_need_no_positions(lens, T, H, kvh, hd, ring, q_pad, kv_pad):
+    """qkv_post_tree without positions against the same with lens + i, and both
+    against qkv_post with a cache per row; rows further apart than they are long."""
+    rng = np.random.default_rng(T + hd)
+    rows, n = len(lens), len(lens) * T
+    cap = ring + 2 if ring else max(lens) + T - 3 if T > 3 else max(lens) + T  # some past the end
+    pos = (np.array(lens, np.int32)[:, None] + np.arange(T, dtype=np.int32)).reshape(-1)
+    ld = dev(np.array(lens, np.int32))
+    qn, kn = (dev(rng.uniform(0.5, 1.5, hd).astype(np.float32)) for _ in range(2))
+    inv = (1.0 / 10000.0 ** (np.arange(0, hd, 2) / hd)).astype(np.float32)
+    cs = dev(D.rope_table(60, hd, inv))  # shorter than the positions
+    x = [rng.standard_normal((n, w)).astype(np.float32)
+         for w in (H * hd + q_pad, kvh * hd + kv_pad, kvh * hd + kv_pad)]
+    got = []
+    for p in (dev(pos), None):
+        c = Cache(np.random.default_rng(1), rows, cap, kvh, hd, ring)
+        kv = c.put()
+        a = [dev(t) for t in x]
+        D.qkv_post_tree(kv, *a, H, T, qn, kn, 1e-6, dev(inv), p, ld, q_ld=H * hd + q_pad,
+                        kv_ld=kvh * hd + kv_pad, cs=cs)
+        got.append((a, c))
+    (a, c), (a2, c2) = got
+    assert all(torch.equal(s, t) for s, t in zip(a, a2))
+    assert all(torch.equal(c.d[k].view(torch.uint8), c2.d[k].view(torch.uint8)) for k in c.d)
+    # one cache per row, the slot being the position (0 where it is past 300)
+    each = Cache(rng, n, 300, kvh, hd)
+    each.put()
+    d, at, w = each.d, np.where(pos < 300, pos, 0), [dev(t) for t in x]
+    D.qkv_post(*w, n, H, kvh, hd, qn, kn, 1e-6, dev(inv), dev(pos), 0, 300, d["kc"],
+               d["kc"].stride(0), d["ks"], 300, d["vt"], d["vt"].stride(0), d["vs"], 300, cs=cs,
+               q_ld=H * hd + q_pad, kv_ld=kvh * hd + kv_pad)
+    assert all(torch.equal(s, t) for s, t in zip(a, w))
+    kd = d["kc"].cpu().numpy()
+    vt = d["vt"].cpu().numpy().reshape(n, 75, kvh * hd, 4)
+    ks, vs = d["ks"].cpu().numpy(), d["vs"].cpu().numpy()
+    sure = np.zeros((rows, cap), bool)  # slots whose row the caches per row can tell
+    sure[:] = True
+    for r in range(n):
+        s = pos[r] % ring if ring else pos[r]
+        if s >= cap:
+            continue
+        sure[r // T, s] = pos[r] < 300
+        p = at[r]
+        c.k[r // T, s], c.v[r // T, s] = kd[r, p], vt[r, p // 4, :, p % 4]
+        c.ks[r // T, s], c.vs[r // T, s], c.tpos[r // T, s] = ks[r, p], vs[r, p], pos[r]
+    assert np.array_equal(c.d["kc"].cpu().numpy()[sure], c.k[sure])
+    got_v = c.d["vt"].cpu().numpy().reshape(rows, -1, kvh * hd, 4).transpose(0, 1, 3, 2)
+    assert np.array_equal(got_v.reshape(rows, -1, kvh * hd)[:, :cap][sure], c.v[:, :cap][sure])
+    for name in ("ks", "vs"):
+        assert np.array_equal(c.d[name].cpu().numpy()[sure], getattr(c, name)[sure])
+    assert np.array_equal(c.d["tpos"].cpu().numpy(), c.tpos)

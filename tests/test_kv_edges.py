@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import fastgemma_b200.device as D
-from test_kv_tree import Cache, check_attend, dev, run_attend, setup
+from test_kv_tree import EPS, Cache, accum64, attend64, check_attend, dev, run_attend, setup
 
 torch = pytest.importorskip("torch")
 gpu = pytest.mark.gpu
@@ -174,3 +174,91 @@ def test_chain_rows_need_no_positions(lens, T, H, kvh, hd, ring, q_pad, kv_pad):
     for name in ("ks", "vs"):
         assert np.array_equal(c.d[name].cpu().numpy()[sure], getattr(c, name)[sure])
     assert np.array_equal(c.d["tpos"].cpu().numpy(), c.tpos)
+
+
+# --------------------------------------------------------- large batches
+def many(rng, rows, most):
+    """Lengths of every size up to `most`, among them 0 and `most`."""
+    lens = np.exp(rng.uniform(0, np.log(most), rows)).astype(int)
+    lens[rows // 2], lens[-1] = 0, most
+    return lens.tolist()
+
+
+@gpu
+@pytest.mark.parametrize("rows,T,H,kvh,hd,kind,window,most", [
+    (33, 2, 4, 2, 64, "tree", 0, 700), (64, 3, 8, 4, 128, "chain", 0, 2500),
+    (100, 1, 2, 1, 256, "chain", 50, 300), (70, 5, 8, 2, 64, "tree", 90, 1500),
+    (33, 20, 4, 2, 64, "tree", 0, 1500), (64, 40, 8, 8, 64, "any", 0, 400),
+    (70, 33, 2, 1, 128, "tree", 120, 1300), (40, 17, 2, 2, 320, "chain", 0, 600)])
+def test_batches_of_more_sequences_than_a_warp_has_lanes(rows, T, H, kvh, hd, kind, window, most):
+    """Ragged batches, from fewer items than SMs to several times as many, with
+    few and with many query rows per KV head; attention, then its weights."""
+    rng = np.random.default_rng(rows * T + hd)
+    lens = many(rng, rows, most)
+    cache, q, mask, pos = setup(rng, lens, T, H, kvh, hd, kind, window)
+    (kv, qd, ld, w, pd, _, lse), weights, S = check_attend(cache, q, H, T, lens, mask, pos, window)
+    take = rng.integers(0, 2, (rows, T)).astype(np.uint8)
+    want = accum64(cache, weights, T, lens, take, np.float32(0.9), None)
+    D.attend_accum_q8(qd, kv, H, T, ld, lse, mask=w, pos=pd, window=window, take=dev(take), decay=0.9)
+    got = cache.d["acc"].cpu().numpy()
+    tol = (32 * S + 128 + (most + T) / 8 + T * H) * EPS
+    assert (np.abs(got - want) <= tol * np.maximum(np.abs(want), 1)).all()
+    for b, n in enumerate(lens):
+        assert np.array_equal(got[b, n + T:], cache.acc[b, n + T:])
+
+
+@gpu
+@pytest.mark.parametrize("rows,H,kvh,hd,most", [(33, 4, 2, 64, 900), (100, 8, 1, 256, 300),
+                                                (70, 16, 4, 128, 1500)])
+def test_decode_step_of_more_sequences_than_a_warp_has_lanes(rows, H, kvh, hd, most):
+    rng = np.random.default_rng(rows)
+    lens = many(rng, rows, most)
+    cache, q, _, pos = setup(rng, lens, 1, H, kvh, hd, "chain")
+    want, _, weights, S, V = attend64(cache, q, H, 1, lens, None, pos, 0)
+    kv, out = cache.put(), torch.empty(rows, H * hd, device="cuda")
+    D.attend_acc_q8(out, dev(q), kv, H, dev(np.array(lens, np.int32)), decay=0.75)
+    tol = (16 * S + 64 + (most + 1) / 8) * EPS
+    assert np.abs(out.cpu().numpy() - want).max() <= tol * V
+    acc = accum64(cache, weights, 1, lens, None, 0.75, None)
+    got = cache.d["acc"].cpu().numpy()
+    assert (np.abs(got - acc) <= (2 * tol + H * EPS) * np.maximum(acc, 1)).all()
+
+
+@gpu
+@pytest.mark.parametrize("T", [1, 17])
+def test_more_items_than_a_launch_splits(T):
+    """130 sequences of 128 KV heads: an item a CTA, whatever its length."""
+    rng = np.random.default_rng(T)
+    rows, H, hd, most = 130, 128, 64, 140
+    lens = many(rng, rows, most)
+    cache, q, _, pos = setup(rng, lens, T, H, H, hd, "chain")
+    kv, qd, ld, _, pd, out, lse = run_attend(cache, q, H, T, lens, None, pos, 0)
+    want, wlse, acc = np.zeros((rows * T, H, hd)), np.zeros((rows * T, H)), cache.acc.astype(float)
+    S = V = 0.0
+    for b, n in enumerate(lens):
+        qb = q[b * T:(b + 1) * T].reshape(T, H, hd)
+        top = np.abs(qb).max(-1, keepdims=True)
+        q8 = np.clip(np.rint(qb * (np.float32(127) / top)), -127, 127).astype(np.float64)
+        k = cache.k[b, :n + T].reshape(-1, H, hd) * cache.ks[b, :n + T, None, None].astype(float)
+        v = cache.v[b, :n + T].reshape(-1, H, hd) * cache.vs[b, :n + T, None, None].astype(float)
+        s = np.einsum("thd,nhd->thn", q8 * (top / np.float32(127)).astype(float), k)
+        s[~np.broadcast_to((np.arange(n + T) <= n + np.arange(T)[:, None])[:, None], s.shape)] = -np.inf
+        m = s.max(-1, keepdims=True)
+        e = np.exp(s - m)
+        p = e / e.sum(-1, keepdims=True)
+        want[b * T:(b + 1) * T] = np.einsum("thn,nhd->thd", p, v)
+        wlse[b * T:(b + 1) * T] = (m + np.log(e.sum(-1, keepdims=True)))[..., 0]
+        acc[b, :n + T] = np.where(np.arange(n + T) < n, 0.5 * acc[b, :n + T], 0) + p.sum((0, 1))
+        S, V = max(S, np.abs(s[np.isfinite(s)]).max()), max(V, np.abs(v).max())
+    tol = (16 * S + 64 + (most + T) / 8) * EPS
+    assert np.abs(out.cpu().numpy() - want.reshape(rows * T, -1)).max() <= tol * V
+    assert (np.abs(lse.cpu().numpy() - wlse) <= tol * np.maximum(1, np.abs(wlse))).all()
+    bound = (2 * tol + T * H * EPS) * np.maximum(acc, 1)
+    D.attend_accum_q8(qd, kv, H, T, ld, lse, pos=pd, decay=0.5)
+    assert (np.abs(cache.d["acc"].cpu().numpy() - acc) <= bound).all()
+    if T == 1:
+        cache.d["acc"].copy_(dev(cache.acc))
+        one = torch.empty_like(qd)
+        D.attend_acc_q8(one, qd, kv, H, ld, decay=0.5)
+        assert np.abs(one.cpu().numpy() - want.reshape(rows, -1)).max() <= tol * V
+        assert (np.abs(cache.d["acc"].cpu().numpy() - acc) <= bound).all()

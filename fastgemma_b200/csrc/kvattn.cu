@@ -58,6 +58,24 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// The same into fresh registers: D = A * B.
+__device__ __forceinline__ void mma_f16_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                            uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+// (a, b) += (c, d): the packed form of the FP32 pipe.
+__device__ __forceinline__ void add_pair(float &a, float &b, float c, float d) {
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\t"
+      "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(a), "+f"(b)
+      : "f"(c), "f"(d));
+}
+
 // ------------------------------------------------------- few rows: streaming
 // Up to 8 * NT query rows against a stream of K and V: bound by reading the
 // cache.  Every warp runs on its own: a private ring of 16-slot stages filled
@@ -68,14 +86,21 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
 // the slot-interleaved V is a lane's four slots of one dimension: V needs no
 // shuffling, only its conversion to f16, which is exact.  A weight p * vs is
 // split into two f16 (scaled by a running power of two above the largest
-// |vs|), 22 bits in all, so the products lose less than f32 rounding does.
+// |vs|), 22 bits in all, so the products lose less than f32 rounding does.  The
+// tensor cores round a sum towards zero, which adds up over a long run (a warp's
+// 512 steps over 64K slots: 1e-5 of the output's norm), so a step's product starts
+// from zero, its small part first, and is added to the output by rounding to nearest
+// (1.8e-6; at 16K slots of head_dim 64 0.5e-6 against 1.5e-6; with equal weights
+// and positive values a mean error of 3e-8 instead of 5e-5).  That costs 1 to 2 %
+// where reading bounds the call, 6 % at head_dim 512, 8 % with 16 rows of 256 and
+// 19 % at 320 (8 sequences of 16K slots; 16 of 20K).
 //
-// 8 sequences of up to 32K slots, 8 heads over 2 of head_dim 256: 50 us for
-// 212 MB (4.2 TB/s over the launch, 6 to 7 while the rings run; 36 % of the
+// 8 sequences of up to 32K slots, 8 heads over 2 of head_dim 256: 51 us for
+// 212 MB (4.1 TB/s over the launch, 6 to 7 while the rings run; 36 % of the
 // issue slots, 18 % of the tensor cycles): 6 us before the first stage has
 // landed, up to 6 % longer runs on some CTAs, 3 to 5 for a join.  Two CTAs an
 // SM with rings of half the length took 54.  Short calls are latency: 4 nodes
-// over 96 slots 9.7 us.
+// over 96 slots 10.1 us.
 constexpr int kTile = 128;   // slots per tile of the work list
 constexpr int kStep = 16;    // slots per warp step
 // Tiles of an item that one CTA takes alone: another tile there against the
@@ -351,18 +376,25 @@ __global__ void __launch_bounds__(stream_warps(HD) * 32, 1)
       uint32_t lo[4], hi[4];
 #pragma unroll
       for (int i = 0; i < 4; i++) i8x4_to_f16(vw[i], lo[i], hi[i]);
+      float t[2][NT][4];
 #pragma unroll
       for (int i = 0; i < 2; i++)
 #pragma unroll
         for (int n = 0; n < NT; n++)
-          mma_f16(o[n][2 * j + i], lo[2 * i], lo[2 * i + 1], hi[2 * i], hi[2 * i + 1], bh[n][0],
-                  bh[n][1]);
+          mma_f16_new(t[i][n], lo[2 * i], lo[2 * i + 1], hi[2 * i], hi[2 * i + 1], bl[n][0],
+                      bl[n][1]);
 #pragma unroll
       for (int i = 0; i < 2; i++)
 #pragma unroll
         for (int n = 0; n < NT; n++)
-          mma_f16(o[n][2 * j + i], lo[2 * i], lo[2 * i + 1], hi[2 * i], hi[2 * i + 1], bl[n][0],
-                  bl[n][1]);
+          mma_f16(t[i][n], lo[2 * i], lo[2 * i + 1], hi[2 * i], hi[2 * i + 1], bh[n][0], bh[n][1]);
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int e = 0; e < 4; e += 2)
+            add_pair(o[n][2 * j + i][e], o[n][2 * j + i][e + 1], t[i][n][e], t[i][n][e + 1]);
     }
     __syncwarp();
     stage = stage + 1 == S ? 0 : stage + 1;

@@ -262,3 +262,44 @@ def test_more_items_than_a_launch_splits(T):
         D.attend_acc_q8(one, qd, kv, H, ld, decay=0.5)
         assert np.abs(one.cpu().numpy() - want.reshape(rows, -1)).max() <= tol * V
         assert (np.abs(cache.d["acc"].cpu().numpy() - acc) <= bound).all()
+
+
+# ----------------------------------------------------- sums over long runs
+@gpu
+@pytest.mark.parametrize("T,tol", [(1, 2 * 34 + 16)])
+def test_long_sums_are_not_rounded_towards_zero(T, tol):
+    """Equal weights over positive values, every item of 128 on one CTA: sums
+    that grow all along.  An instruction of the tensor cores may cut each of its
+    16 products and what it adds them to down to 2^-23 of the sum, 17 units, so an
+    accumulator that takes all of a run loses a part that grows with the run.
+    Rounding to nearest has no mean error; what the mean over all outputs may be
+    off is the units of two instructions on one step's sum (streaming kernel) and 16 *
+    2^-24 for the weights' 22 bits, the division and the scaling.  The sum of
+    the weights is exact."""
+    n = 65536
+    g = torch.Generator(device="cuda").manual_seed(n)
+    rows, kvh, G, hd, cap = 16, 8, 8, 64, n + 4
+    kvd = kvh * hd
+    kc = torch.zeros(rows, cap, kvd, dtype=torch.int8, device="cuda")
+    vt = torch.randint(64, 128, (rows, cap // 4, kvd, 4), dtype=torch.int8, device="cuda", generator=g)
+    ks = torch.ones(rows, cap, device="cuda")
+    vs = torch.rand(rows, cap, device="cuda", generator=g) * 0.5 + 0.5
+    kv = D.KvCache(kc, ks, vt, vs, kvh, hd, acc=torch.zeros(rows, cap, device="cuda"))
+    q = torch.zeros(rows * T, kvh * G * hd, device="cuda")
+    lens = torch.full((rows,), n, dtype=torch.int32, device="cuda")
+    out = torch.empty_like(q)
+    D.attend_tree_q8(out, q, kv, kvh * G, T, lens)
+    got = out.double().reshape(rows, T, kvh, G, hd)
+    want = torch.empty(rows, T, kvd, dtype=torch.float64, device="cuda")
+    for b in range(rows):
+        x = vt[b].double() * vs[b].double().reshape(-1, 1, 4)
+        x = x.transpose(1, 2).reshape(cap, kvd)
+        for i in range(T):
+            want[b, i] = x[:n + i + 1].sum(0) / (n + i + 1)
+    off = got / want.reshape(rows, T, kvh, 1, hd) - 1
+    assert abs(off.mean().item()) <= tol * EPS
+    if T == 1:
+        one = torch.empty_like(q)
+        D.attend_acc_q8(one, q, kv, kvh * G, lens)
+        off = one.double().reshape(got.shape) / want.reshape(rows, T, kvh, 1, hd) - 1
+        assert abs(off.mean().item()) <= tol * EPS

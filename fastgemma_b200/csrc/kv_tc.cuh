@@ -89,6 +89,18 @@ __device__ __forceinline__ void bulk_s2g(void *dst, const void *src, uint32_t by
                : "memory");
 }
 
+// Adds four f32 to memory, each rounded to nearest, without waiting.
+__device__ __forceinline__ void red_add4(float4 *to, float4 v) {
+  asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(to), "f"(v.x),
+               "f"(v.y), "f"(v.z), "f"(v.w)
+               : "memory");
+}
+
+// Orders plain accesses to global memory before later bulk copies.
+__device__ __forceinline__ void fence_proxy_async_global() {
+  asm volatile("fence.proxy.async.global;" ::: "memory");
+}
+
 __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }

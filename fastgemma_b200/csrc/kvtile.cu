@@ -20,19 +20,27 @@
 // over CTAs are joined by a kernel after.
 //
 // A tile costs 128 * 128 * hd MACs at the int8 rate and twice that at the f16
-// rate, 1.45 us at head_dim 256, and takes 3.0: the MMAs, in the order of their
-// issue, the softmax (2.5 us) and the conversion (2.6 us, half of it waiting
-// for loads and stores to land) each wait for the others once per tile.  Left
-// out one at a time they gain 3 us (conversion) and 7 us (softmax) of 65, both
-// together 18.  Beside the tiles a call costs 23 us: the quantisation 4, setup
-// 3 (under it), the way to the first weights 4, the last product and 128 KB of
+// rate, 1.45 us at head_dim 256, and takes 3.0 (3.45 with the drains below):
+// the MMAs, in the order of their issue, the softmax (2.5 us) and the
+// conversion (2.6 us, half of it waiting for loads and stores to land) each wait
+// for the others once per tile.  Left out one at a time they gained 3 us
+// (conversion) and 7 us (softmax) of 65, both together 18, before there were
+// drains.  Beside the tiles a call costs 23 us: the quantisation 4, setup 3
+// (under it), the way to the first weights 4, the last product and 128 KB of
 // partial results a CTA 5, the join 4, the rest launches.  256 nodes, 8 heads
-// over 2, head_dim 256: 65.2 us over 16K slots, 191 over 64K (720 TFLOP/s of
+// over 2, head_dim 256: 74.5 us over 16K slots, 218 over 64K (630 TFLOP/s of
 // the two products; each counted once).
 //
-// Accuracy: the tensor cores add into the f32 output without rounding to
-// nearest, sixteen times per tile; over fifteen tiles that is 2.9e-6 of the
-// output's norm, where rounding every f32 step leaves 1.7e-6.
+// Accuracy: the tensor cores cut an f32 sum off instead of rounding it, sixteen
+// times per tile, for each term that is added; over a run of 512 tiles of equal
+// weights and positive values that came to 4e-4 of the output (1.2e-6 now), over 57
+// tiles of random ones to 1e-5 of its norm.  So the output is drained every kDrain tiles
+// into memory (L2 holds it), where the parts are added with rounding to nearest,
+// and the products start anew.  Error of random values at any length, and 256
+// nodes over 64K slots: without drains 1e-5 and 183 us; every 8 tiles 1.7e-6 and
+// 201; 6: 1.4e-6, 206; 4: 1.0e-6, 217, which is what rounding every f32 step leaves;
+// 3: 0.8e-6, 231.  A drain costs 2.2 us, 1.4 of them the stores, the first 2
+// more for the join at the end.
 #include <type_traits>
 
 #include "kv_tc.cuh"
@@ -48,6 +56,7 @@ constexpr int kSoftWarps = 16, kSoft = kSoftWarps * 32;
 constexpr int kThreads = 128 + kSoft + 128;  // loads and MMAs, softmax, V conversion
 constexpr int kQuarter = kTN / 4;  // slots of a softmax thread
 constexpr int kGrow = 8;          // log2 by which a row's maximum may grow unnoticed
+constexpr int kDrain = 4;         // tiles between two drains of the output, at most
 constexpr int kUnit = 7;          // f16 weights: p * vs * 2^(kUnit - ve), below 2^(kUnit + kGrow)
 // TMEM columns: output [0, 256), scores 128, weights of 64 slots 2 x (32 high, 32 low parts)
 constexpr uint32_t kColS = 256, kColP = 384;
@@ -101,6 +110,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   const float *vs = p.kv.vs + (size_t)b * p.kv.vs_stride;
 
   const int chunks = tiles * tp.nkb, halves = tiles * 2;
+  // The run in segments of kDrain tiles, with a drain between; what is short of
+  // whole ones is missing in the first or the last, by CTA, so that not all CTAs
+  // drain at once (16 sequences, 8 KV heads, 16K slots: 642 us against 658).
+  const int spare = (tiles + kDrain - 1) / kDrain * kDrain - tiles;
+  const int first = kDrain - (int)blockIdx.x % (spare + 1);
   auto load_k = [&](int c) {  // chunk c: tile c / nkb, bytes 128 * (c % nkb) of the rows
     const int st = c % tp.kstages, t = c / tp.nkb;
     tc::mbar_expect_tx(&bar.k_full[st], kChunk);
@@ -202,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t id_s = tc::idesc_i8(kTM, kTN), id_o = idesc_f16(kTM, dv);
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
     const int n = __shfl_sync(0xffffffffu, tiles, 0);
-    int kst = 0, vst = 0;
+    int kst = 0, vst = 0, left = __shfl_sync(0xffffffffu, first, 0);
     uint32_t kph = 0, vph = 0;
     auto scores = [&] {
       const uint32_t d = tm + kColS;
@@ -231,6 +245,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         wait(&bar.s_empty, j & 1);
         scores();
       }
+      const bool fresh = j == 0 || left == kDrain;  // the output starts anew
+      left = left == 1 ? kDrain : left - 1;
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         wait(&bar.p_full[h], j & 1);
@@ -241,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (elected()) {
 #pragma unroll
           for (int k = 0; k < 4; k++) {
-            mma_f16_ts(tm, a + k * 8, v + k * 2, id_o, j + h + k > 0);
+            mma_f16_ts(tm, a + k * 8, v + k * 2, id_o, !fresh || h + k > 0);
             mma_f16_ts(tm, a + 32 + k * 8, v + k * 2, id_o, 1);
           }
           tc::mma_commit(&bar.v_empty[vst]);
@@ -331,7 +347,58 @@ __global__ void __launch_bounds__(kThreads, 1)
     meet();
     float m = -INFINITY, l = 0.0f;
 
-    auto tile = [&](int j, auto is_masked) {
+    // The output after a segment added to what was drained before, under the
+    // maximum `ref` of the row's first segment until it has grown by 2^60.  Four
+    // dimensions of the quadrant's 32 rows follow one another, so that a warp's
+    // stores are whole lines; the place is that of the CTA's partial results of
+    // these rows.  It comes after the next tile's weights are stored, by when
+    // the segment's last product is done and the scores' registers are free, and
+    // before they are handed over.  64K slots: 217 us; ahead of the next tile's
+    // softmax 230; by the conversion's warps 293, by warps 0 to 3 241 (registers
+    // pushed out to memory).
+    float4 *drained = reinterpret_cast<float4 *>(
+        tp.part + ((size_t)blockIdx.x * kTM + (warp & 3) * 32) * dv) + lane;
+    float ref = -INFINITY;
+    bool some = false;
+    auto drain = [&](int j, float top) {
+      wait(&bar.p_empty[0], j & 1);
+      wait(&bar.p_empty[1], j & 1);
+      tc::fence_after_sync();
+      if (ref == -INFINITY) ref = top;  // only zeros so far
+      float scale = ref == -INFINITY ? 1.0f : ex2(top - ref), g = 1.0f;
+      const bool far = some && __any_sync(0xffffffffu, scale > pow2(60));
+      if (far) {
+        g = ref == -INFINITY ? 1.0f : ex2(ref - top);
+        ref = top;
+        scale = 1.0f;
+      }
+      for (int c = quarter * (dv / 4); c < (quarter + 1) * (dv / 4); c += 8) {
+        uint32_t o[8];
+        tmem_ld_x8(quad + c, o);
+        tc::tmem_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 8; k += 4) {
+          float4 *to = drained + (c + k) * 8;  // (c + k) / 4 groups of 32 rows
+          const float4 v = make_float4(
+              __uint_as_float(o[k]) * scale, __uint_as_float(o[k + 1]) * scale,
+              __uint_as_float(o[k + 2]) * scale, __uint_as_float(o[k + 3]) * scale);
+          if (!some) {
+            __stcg(to, v);
+          } else if (!far) {
+            red_add4(to, v);
+          } else {
+            const float4 a = __ldcg(to);
+            __stcg(to, make_float4(__fmaf_rn(a.x, g, v.x), __fmaf_rn(a.y, g, v.y),
+                                   __fmaf_rn(a.z, g, v.z), __fmaf_rn(a.w, g, v.w)));
+          }
+        }
+      }
+      tc::fence_before_sync();
+      meet();
+      some = true;
+    };
+
+    auto tile = [&](int j, bool fresh, auto is_masked) {
       constexpr bool masked = decltype(is_masked)::value;
       const int buf = j & 1;
       const float *ksq = s_ks[buf] + quarter * kQuarter, *vsq = s_vs[buf] + quarter * kQuarter;
@@ -388,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         m = top;
         l *= f;
       }
-      if (__any_sync(0xffffffffu, f != 1.0f)) {
+      if (!fresh && __any_sync(0xffffffffu, f != 1.0f)) {
         wait(&bar.p_empty[0], (j - 1) & 1);
         wait(&bar.p_empty[1], (j - 1) & 1);
         tc::fence_after_sync();
@@ -450,17 +517,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_st_x16(to + 32, lo);
       tmem_wait_st();
     };
-    for (int j = 0; j < tiles; j++) {
+    for (int j = 0, left = first; j < tiles; j++) {
+      const bool fresh = j == 0 || left == kDrain;  // its products add to nothing
+      left = left == 1 ? kDrain : left - 1;
       wait(&bar.sc_full[j & 1], (j >> 1) & 1);
       wait(&bar.s_full, j & 1);
       tc::fence_after_sync();
       if (idle) {
         if (lane == 0) tc::mbar_arrive(&bar.s_empty);
         if (j > 0) wait(&bar.p_empty[quarter >> 1], (j - 1) & 1);
-      } else if (ring || x0 + (j + 1) * kTN > len || x0 + j * kTN < high) {
-        tile(j, std::true_type());
       } else {
-        tile(j, std::false_type());
+        const float was = m;
+        if (ring || x0 + (j + 1) * kTN > len || x0 + j * kTN < high)
+          tile(j, fresh, std::true_type());
+        else
+          tile(j, fresh, std::false_type());
+        if (fresh && j > 0) drain(j - 1, was);
       }
       tc::fence_before_sync();
       __syncwarp();
@@ -478,6 +550,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     wait(&bar.p_empty[1], (tiles - 1) & 1);
     tc::fence_after_sync();
     const bool whole = wk.count == 1;
+    const float g = ref == -INFINITY ? 0.0f : ex2(ref - m);
     float back = pow2(ve) * 0.0078125f;  // 2^-kUnit
     if (whole) back = L == 0.0f ? 0.0f : back / L;
     float *stage = reinterpret_cast<float *>(sm + (size_t)row * (dv * 4 + 16));
@@ -489,6 +562,18 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int e = 0; e < 4; e++) tmem_ld<N>(quad + e * (dv / 4) + i, o[e]);
         tc::tmem_wait_ld();
+        if (some) {
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (int k = 0; k < N; k += 2) {
+              const int c = e * (dv / 4) + i + k;
+              const float2 a =
+                  __ldcg(reinterpret_cast<const float2 *>(drained + c / 4 * 32) + (c / 2 & 1));
+              o[e][k] = __float_as_uint(__fmaf_rn(a.x, g, __uint_as_float(o[e][k])));
+              o[e][k + 1] = __float_as_uint(__fmaf_rn(a.y, g, __uint_as_float(o[e][k + 1])));
+            }
+        }
 #pragma unroll
         for (int k = 0; k < N; k++)
           *reinterpret_cast<float4 *>(stage + 4 * (i + k)) =
@@ -503,6 +588,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       put(std::integral_constant<int, 2>());
     }
     tc::fence_before_sync();
+    if (some) fence_proxy_async_global();  // the copy below goes where the drained rows lie
     stream::fence_proxy_async_smem();
     meet();
     if (quarter == 0 && row < rows) {

@@ -266,14 +266,15 @@ def test_more_items_than_a_launch_splits(T):
 
 # ----------------------------------------------------- sums over long runs
 @gpu
-@pytest.mark.parametrize("T,tol", [(1, 2 * 34 + 16)])
+@pytest.mark.parametrize("T,tol", [(1, 2 * 34 + 16), (3, 2 * 17 * 33 + 16)])
 def test_long_sums_are_not_rounded_towards_zero(T, tol):
     """Equal weights over positive values, every item of 128 on one CTA: sums
     that grow all along.  An instruction of the tensor cores may cut each of its
     16 products and what it adds them to down to 2^-23 of the sum, 17 units, so an
     accumulator that takes all of a run loses a part that grows with the run.
     Rounding to nearest has no mean error; what the mean over all outputs may be
-    off is the units of two instructions on one step's sum (streaming kernel) and 16 *
+    off is the units of two instructions on one step's sum (streaming kernel), or
+    of 64 on the growing sum of four tiles (tile kernel, 17 * 33 units), and 16 *
     2^-24 for the weights' 22 bits, the division and the scaling.  The sum of
     the weights is exact."""
     n = 65536

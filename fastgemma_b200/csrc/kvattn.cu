@@ -639,13 +639,21 @@ cudaError_t launch_stream(const TreeParams &p, bool accumulate, int num_sms, cud
 
 }  // namespace
 
-// The streaming kernel up to 16 query rows per KV head, where the cache's bytes
-// bound the work; beyond, the tensor tiles, except over caches so short that
-// the row blocks of 16 fit the SMs at once and run their few slots through
-// before a tile kernel's three launches would be done: at 230 slots of head_dim
-// 256 and 64 rows for each of 8 sequences 12.8 against 17.1 us, at 990 slots
-// 23.5 against 19.1; at 990 of head_dim 64 14.0 against 17.3, at 4000 24.2
-// against 24.0.
+// The streaming kernel up to 16 query rows per KV head; beyond, the tensor
+// tiles, except over caches so short that the row blocks of 16 fit the SMs at
+// once and run their few slots through before a tile kernel's three launches
+// would be done: at 230 slots of head_dim 256 and 64 rows for each of 8 sequences
+// 13.1 against 17.9 us, at 990 slots 23.9 against 19.4; at 990 of head_dim 64 14.5
+// against 17.4, at 4000 24.9 against 23.7.
+//
+// Up to 16 rows, streaming against tiles, two KV heads, 16K slots: 4 rows of
+// head_dim 256 17.1 against 26.6 us for one sequence, 34.3 against 63.1 for
+// eight; 16 rows of 64 17.2 against 25.4 and 24.8 against 47.1.  The number of rows
+// alone is a coarse rule: at 16 rows of 256 the tiles are ahead for one sequence
+// (27.3 against 31.7) and behind for eight (63.8 against 55.7), and from 1000 slots
+// on they are ahead for one sequence of head_dim 320 and more from 8 rows on (512:
+// 30.3 against 47.4) and for eight of 512 with 16 rows (118.8 against 141.1),
+// where the stream runs four warps and reads the cache once per 8 rows.
 bool streams(const TreeParams &p) {
   const int R = p.T * (p.n_heads / p.kv.kv_heads);
   if (R <= 16) return true;

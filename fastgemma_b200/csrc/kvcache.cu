@@ -85,13 +85,14 @@ struct AcceptParams {
   int32_t *lens_new;
 };
 
-// One CTA per (sequence, layer); bound by the latency of lens, path, rows (3.7
-// us with the verification for one sequence and 4 layers, 6.6 for 8 sequences of
-// 61 nodes and 30 layers).  Warp 0 moves K rows, 16 bytes a lane, the
-// others V, a dimension's word a lane, eight path entries at a time: their
-// loads all go out before the first store.  That keeps the order right too:
-// the destination of entry j lies at or before its source and the sources
-// ascend, so no store of a batch lands on a row that a later entry still reads.
+// One CTA per (sequence, layer); bound by the latency of lens, path, rows (4.2
+// us with the verification for one sequence and 4 layers, 7.1 for 8 sequences of
+// 61 nodes and 30 layers, in a graph; as two ordinary calls the host needs 14).
+// Warp 0 moves K rows, 16 bytes a lane, the others V, a dimension's word a lane,
+// eight path entries at a time: their loads all go out before the first store.
+// That keeps the order right too: the destination of entry j lies at or before
+// its source and the sources ascend, so no store of a batch lands on a row that
+// a later entry still reads.
 constexpr int kAcceptBatch = 8;
 __global__ void __launch_bounds__(256) kv_accept_kernel(const __grid_constant__ AcceptParams p) {
   __shared__ int s_from[kTreeMax], s_to[kTreeMax], s_n;

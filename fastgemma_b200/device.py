@@ -324,7 +324,9 @@ def tree_mask(mask, pos, parent, lens, stream=None):
 def attend_tree_q8(out, q, kv, n_heads, T, lens, mask=None, pos=None, window=0, lse=None, ws=None,
                    q_ld=None, out_ld=None, stream=None):
     """T nodes of each sequence attend to its cache and to one another (mask
-    None: to the nodes before them); lse [rows * T][n_heads], of any strides, if wanted."""
+    None: to the nodes before them); lse [rows * T][n_heads], of any strides, if
+    wanted.  A window goes by the slots' indexes, so not with a cache that
+    kv_evict_q8 has moved rows in."""
     _flat(lens=lens, mask=mask, pos=pos)
     _rows(q=q, out=out)
     lse = _lse(lse, kv.rows * T, n_heads)

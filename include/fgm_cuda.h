@@ -479,14 +479,20 @@ size_t fgm_cuda_attend_workspace(const fgm_cuda_kv *kv, int n_heads, int T);
  * Node i sees every committed slot and the nodes j whose bit is set in mask
  * (fgm_cuda_tree_mask's words; bits past T do not matter), or, when mask is
  * NULL, the nodes j <= i.  window > 0: of these only the positions above
- * pos[b*T + i] - window, a committed slot's position being its own and node
- * j's being pos[b*T + j]; pos NULL means lens[b] + i.
+ * pos[b*T + i] - window, a committed slot's position being the one it has by
+ * its index (tpos is not read, so a cache that fgm_cuda_kv_evict_q8 has moved
+ * rows in takes no window) and node j's being pos[b*T + j]; pos NULL means
+ * lens[b] + i.
  * Per head: q8 = rint(q * (127 / max|q|)), score = (q8 . k8) * (max|q| / 127)
  * * ks[slot] as in fgm_cuda_attend_q8; out = sum(softmax(score) * vs * v8)
  * with the weights in f32 (attend_q8 rounds them to 16 bits, as the
  * reference does, so the two differ by that), scaled by the largest |vs| that
  * one thread block meets: a slot whose |vs| is 2^13 times below that one's
- * weighs with 17 bits or more, still smaller ones with fewer.  A node that
+ * weighs with 17 bits or more, still smaller ones with fewer.  The sums are
+ * f32; the tensor cores cut them off over 16 slots (up to 16 query rows per KV
+ * head, and short caches) or 512 at most and what lies between is rounded to
+ * nearest, so the error does not grow with the cache: about 1e-6 of the
+ * output's norm at most.  A node that
  * sees nothing gets zeros.  lse (may be NULL): log of the sum of exp(score) of
  * row r = b*T + i, head h at lse[r * lse_row + h * lse_head]; -inf for such a
  * node.  A query head with a value that is no finite number gives
@@ -548,9 +554,10 @@ int fgm_cuda_kv_accept(const fgm_cuda_kv *kv, int layers, int T, const int32_t *
  * from (its own index where it stayed, -1 past a cache shorter than the
  * budget); lens_out [rows]: min(lens, budget), may be lens.  tpos NULL: a
  * slot's position is its index.  acc_out / tpos_out: rows of out_stride
- * elements, or NULL: kv->acc and kv->tpos are updated in place.  Linear caches
- * (ring == 0) of at most 524288 slots; kv->acc is needed; 1 <= budget <= cap,
- * sink >= 0, recent >= 0. */
+ * elements, or NULL: kv->acc and kv->tpos are updated in place.  A slot's
+ * index is no longer its token's position then: attention over such a cache
+ * takes no window.  Linear caches (ring == 0) of at most 524288 slots; kv->acc
+ * is needed; 1 <= budget <= cap, sink >= 0, recent >= 0. */
 int fgm_cuda_kv_evict_q8(const fgm_cuda_kv *kv, const int32_t *lens, int budget, int sink,
                          int recent, int32_t *map, int32_t *lens_out, float *acc_out,
                          int32_t *tpos_out, size_t out_stride, void *stream);
